@@ -1,0 +1,111 @@
+// Attention of drafted tokens over the paged cache.  A sequence brings n tokens at once, a tree: their keys and values lie at
+// the cache positions base ... base + n - 1 behind the base tokens that it holds, and token r sees the base tokens (those its
+// window covers, counted from its position) and of the drafted ones those whose bit its mask names - itself and its ancestors:
+//
+//   out[r] = sum_j p[r, j] v[j],  p[r, j] = exp(s[r, j]) / sum over the seen keys,  s = q[r] . k[j] / sqrt(head_dim)
+//
+// A key that a row does not see does not reach it, whatever it holds.  A row that sees nothing gives zeros.
+#include <float.h>
+#include "common.h"
+#include "attention_tree.h"
+#include "yalm_hip.h"
+
+namespace {
+
+// the last sequence whose first row is not behind r
+__device__ __forceinline__ int sequence_of(const int* cu, int B, int r) {
+  int b = 0;
+  for (int hi = B - 1; b < hi;) {
+    const int mid = (b + hi + 1) >> 1;
+    if (cu[mid] <= r) b = mid; else hi = mid - 1;
+  }
+  return b;
+}
+
+// ---------------------------------------------------------------------------
+// Every head size and type, in float32 arithmetic: a wave a (row, head), 64 keys at a time, a lane a key for the scores and a
+// lane an output element for the mix.  For the shapes that the matrix cores' kernel does not take.
+// ---------------------------------------------------------------------------
+constexpr int MAX_HD = 1024;
+
+template <typename T>
+__global__ __launch_bounds__(WAVE) void attn_tree_simple_kernel(TreeArgs a) {
+  constexpr int ACC = MAX_HD / WAVE;
+  __shared__ float qs[MAX_HD];
+  __shared__ float ps[PAGE];
+  const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, hd = a.head_dim;
+  if (r >= a.cu_nodes[a.B]) return;
+  const int b = sequence_of(a.cu_nodes, a.B, r);
+  const TreeSeq s(a, b);
+  T* out = (T*)a.out + ((size_t)r * a.n_heads + h) * hd;
+  const T* q = (const T*)a.q + ((size_t)r * a.n_heads + h) * hd;
+  for (int e = lane; e < hd; e += WAVE) qs[e] = to_f32(q[e]);
+  __syncthreads();
+  const int g = h / (a.n_heads / a.n_kv_heads);
+  const size_t page_elems = (size_t)a.n_kv_heads * PAGE * hd;
+  const int lo = tree_first(a, s, r);
+  const float scale = 1.0f / sqrtf((float)hd);
+  float m = -FLT_MAX, l = 0.f, o[ACC];
+#pragma unroll
+  for (int u = 0; u < ACC; ++u) o[u] = 0.f;
+  for (int page = s.len > 0 ? max(0, min(lo, s.base)) / PAGE : 0; page * PAGE < s.len; ++page) {
+    const int phys = tree_page(a, s, page);
+    const T* kp = (const T*)a.k_pages + phys * page_elems + (size_t)g * PAGE * hd;
+    const T* vp = (const T*)a.v_pages + phys * page_elems + (size_t)g * PAGE * hd;
+    const unsigned long long seen = tree_seen(a, s, r, lo, page);
+    if (seen == 0) continue;
+    float score = -INFINITY;
+    if ((seen >> lane) & 1) {
+      score = 0.f;
+      for (int e = 0; e < hd; ++e) score = fmaf(qs[e], to_f32(kp[page_k_offset(a.page_layout, lane, e, hd)]), score);
+      score *= scale;
+    }
+    const float m_new = fmaxf(m, wave_max(score));
+    const float corr = expf(m - m_new);
+    const float p = (seen >> lane) & 1 ? expf(score - m_new) : 0.f;
+    l = l * corr + wave_sum(p);
+    m = m_new;
+    __syncthreads();
+    ps[lane] = p;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ACC; ++u) {
+      const int e = lane + u * WAVE;
+      if (e >= hd) break;
+      float part = 0.f;
+      for (int j = 0; j < PAGE; ++j)
+        if ((seen >> j) & 1) part = fmaf(ps[j], to_f32(vp[page_v_offset(a.page_layout, j, e, hd)]), part);
+      o[u] = o[u] * corr + part;
+    }
+  }
+  const float inv = l > 0.f ? 1.0f / l : l == l ? 0.f : l;          // a sum that is no number stays one
+#pragma unroll
+  for (int u = 0; u < ACC; ++u) {
+    const int e = lane + u * WAVE;
+    if (e < hd) out[e] = from_f32<T>(o[u] * inv);
+  }
+}
+
+}  // namespace
+
+extern "C" int yalm_attn_tree(const void* q, const void* k_pages, const void* v_pages, const int* block_table, int table_stride,
+                              int n_slots, int ring_pages, const int* seq_slot, const int* seq_len, const int* cu_nodes,
+                              const long long* mask, int mask_words, const int* positions, void* out, float* partial, int T, int B,
+                              int n_heads, int n_kv_heads, int head_dim, int window, int n_splits, int max_nodes, int n_pages,
+                              int page_layout, int dtype, int force_simple, const int* step_max_len, hipStream_t stream) {
+  if (T <= 0 || B <= 0) return YALM_OK;
+  if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || head_dim > MAX_HD || ring_pages <= 0 ||
+      ring_pages > table_stride || n_slots <= 0 || n_pages <= 0 || mask_words <= 0 || n_splits <= 0 || max_nodes <= 0 || n_heads > 65535 ||
+      !page_layout_ok(page_layout, head_dim))
+    return YALM_ERR_ARG;
+  const TreeArgs a = {q, k_pages, v_pages, block_table, table_stride, n_slots, ring_pages, seq_slot, seq_len, cu_nodes,
+                      (const unsigned long long*)mask, mask_words, positions, out, partial, T, B, n_heads, n_kv_heads, head_dim, window,
+                      n_splits, max_nodes, n_pages, page_layout, step_max_len};
+  if (dtype == YALM_F32)
+    attn_tree_simple_kernel<float><<<dim3(T, n_heads), WAVE, 0, stream>>>(a);
+  else if (dtype == YALM_BF16)
+    attn_tree_simple_kernel<bf16><<<dim3(T, n_heads), WAVE, 0, stream>>>(a);
+  else
+    return YALM_ERR_DTYPE;
+  return launch_status();
+}

@@ -304,6 +304,18 @@ int yalm_attn_decode_static(const void* q, const void* k_pages, const void* v_pa
                             int B, int n_heads, int n_kv_heads, int head_dim, int window, int n_splits, int n_pages,
                             int dtype, int force_simple, hipStream_t stream);
 
+// Attention of drafted tokens over the cache (attention_tree.hip).  Sequence b brings the rows cu_nodes[b] ... cu_nodes[b + 1] - 1, at most
+// max_nodes, whose keys and values lie at the last positions below seq_len[b] of slot seq_slot[b] (negative: the rows give zeros); a
+// row sees the sequence's tokens in front of those (window > 0: the ones less than window positions before its own, positions[r], or
+// with null as many places behind them as its mask has bits, less one) and of the drafted ones those whose bits mask[r] (mask_words words of
+// 64 a row) names.  A row that sees no key gives zeros; rows from cu_nodes[B] on are left as they are.  partial: float32, T n_heads
+// n_splits (head_dim + 2) elements, read and written where n_splits > 1.  step_max_len: as in yalm_attn_decode_lse.
+int yalm_attn_tree(const void* q, const void* k_pages, const void* v_pages, const int* block_table, int table_stride, int n_slots,
+                   int ring_pages, const int* seq_slot, const int* seq_len, const int* cu_nodes, const long long* mask, int mask_words,
+                   const int* positions, void* out, float* partial, int T, int B, int n_heads, int n_kv_heads, int head_dim, int window,
+                   int n_splits, int max_nodes, int n_pages, int page_layout, int dtype, int force_simple, const int* step_max_len,
+                   hipStream_t stream);
+
 // out[r] = index of the maximum of logits[r, :], lowest index on ties (src/sampler.cpp:27-38)
 int yalm_argmax(const float* logits, int* out, int R, int V, hipStream_t stream);
 // out[r] = first index whose running sum of exp((l - max)/T) reaches u[r] * total, else V-1
@@ -311,6 +323,26 @@ int yalm_argmax(const float* logits, int* out, int R, int V, hipStream_t stream)
 int yalm_sample(const float* logits, const float* u, float temperature, int* out, int R, int V, hipStream_t stream);
 // prob[r] = softmax(logits[r, :])[index[r]] (src/sampler.cpp:11-25)
 int yalm_token_prob(const float* logits, const int* index, float* prob, int R, int V, hipStream_t stream);
+
+// Sampling under filters (sample_filtered.hip).  With w_i = exp((l_i - max) / temperature[r]), tokens in the order of falling logits and
+// rising indices: K the first top_k[r] of them (0 or less: all), P the shortest prefix of K whose weights reach top_p[r] of K's (1 or
+// more: all of K; at least one), M those of P with w >= min_p[r]; out[r] = the first token of M in the order of the indices at which M's
+// running sum reaches u[r] times its total, prob[r] (may be null) its share of that total.  temperature[r] <= 0: the first of the
+// greatest, probability 1.  No number (NaN) is never drawn; a row without a logit above -infinity gives -1 and 0.  The settings are float32 (top_k
+// int32) [R] on the device; a null pointer stands for temperature 1 or a filter that is off.
+int yalm_sample_filtered(const float* logits, const float* u, const float* temperature, const int* top_k, const float* top_p,
+                         const float* min_p, int* out, float* prob, int R, int V, hipStream_t stream);
+
+// Pages that move (cache_pages.hip).  yalm_copy_blocks: block src[i] of each of the n_lines lines of a (and of b, may be null), lines of
+// n_blocks blocks of block_bytes each, to block dst[i]; no block is a source and another pair's destination; of several copies to
+// one block the last one stands, and numbers outside the lines are passed over.
+// yalm_compact_lines: for sequence b and k < cu_keep[b + 1] - cu_keep[b] (at most max_keep): the key and value at position seq_start[b] +
+// keep[cu_keep[b] + k] to position seq_start[b] + k, in every line of k_pages, v_pages [n_lines][n_pages][...]; keep ascending.
+int yalm_copy_blocks(void* a, void* b, int n_lines, int n_blocks, long block_bytes, const int* src, const int* dst, int n,
+                     hipStream_t stream);
+int yalm_compact_lines(void* k_pages, void* v_pages, const int* block_table, int table_stride, int n_slots, int ring_pages,
+                       const int* seq_slot, const int* seq_start, const int* cu_keep, const int* keep, int B, int n_keep, int max_keep,
+                       int n_lines, int n_pages, int n_kv_heads, int head_dim, int page_layout, int dtype, hipStream_t stream);
 
 // Layers that norm a sublayer's OUTPUT before it joins the residual stream (postnorm.hip).
 // yalm_cast: out[i] = dtype(x[i]).  yalm_norm_add: x[r, :] += y[r, :] * rsqrt(mean(y[r]^2) + eps) * w, and if h_out is

@@ -881,6 +881,63 @@ def attn_decode(q, k_pages, v_pages, block_table, ring_pages, seq_slot, seq_len,
     return out
 
 
+MAX_TREE_NODES = 256             # drafted tokens of a sequence that attn_tree takes
+
+
+def attn_tree_splits(n_seqs, max_nodes, max_len, n_heads, n_kv_heads, head_dim, dtype, window=0):
+    """Into how many pieces attn_tree should cut the keys of a sequence."""
+    return 1
+
+
+def attn_tree_workspace_floats(T, n_heads, head_dim, n_splits):
+    """The float32 elements of attn_tree's `partial` (0: with one split it takes none)."""
+    return T * n_heads * n_splits * (head_dim + 2) if n_splits > 1 else 0
+
+
+def attn_tree(q, k_pages, v_pages, block_table, ring_pages, seq_slot, seq_len, cu_nodes, mask, out, partial, n_heads, n_kv_heads,
+              head_dim, window, n_splits, max_nodes, positions=None, step_max_len=None, layout=None):
+    """Attention of drafted tokens, a tree of them a sequence, over the cache pages that hold the sequence's keys and values and theirs.
+    Sequence b brings the rows cu_nodes[b] ... cu_nodes[b + 1] - 1 of q and out [T, n_heads * head_dim] (rows from cu_nodes[B] on are left as
+    they are), at most max_nodes; its drafted tokens lie at the last positions below seq_len[b].  A row sees the sequence's tokens in front of
+    those, with a window > 0 only the ones less than `window` positions before its own (positions: int32 [T]; None: a row stands as
+    many places behind them as its mask has bits, less one), and of the drafted ones those whose bits its mask names: int64 [T, words],
+    bit j % 64 of word j // 64 for the j-th, itself among them.  What a row does not see does not reach it, whatever it holds; a row that sees
+    nothing, and the rows of a sequence with a negative slot, give zeros.  n_splits: attn_tree_splits; partial: float32, at least
+    attn_tree_workspace_floats elements, not shared with a call that may run at the same time; step_max_len: as in attn_decode."""
+    _check_heads(n_heads, n_kv_heads, head_dim)
+    T = q.shape[0]
+    dt = q.dtype
+    n_pages = k_pages.shape[0]
+    width = (T, n_heads * head_dim)
+    p_q = _need(q, "q", dt, width)
+    p_kp = _need(k_pages, "k_pages", dt, (n_pages, n_kv_heads, PAGE, head_dim))
+    p_vp = _need(v_pages, "v_pages", dt, (n_pages, n_kv_heads, head_dim, PAGE))
+    p_bt = _need(block_table, "block_table", torch.int32, (None, None))
+    n_slots, stride = block_table.shape
+    if ring_pages <= 0 or ring_pages > stride:
+        raise ValueError("ring_pages %d does not fit the block table (%d columns)" % (ring_pages, stride))
+    p_ss = _need(seq_slot, "seq_slot", torch.int32, (None,))
+    B = seq_slot.shape[0]
+    p_m = _need(mask, "mask", torch.int64, (T, None))
+    words = mask.shape[1]
+    if not 1 <= max_nodes <= MAX_TREE_NODES or words < 1 or max_nodes > 64 * words:
+        raise ValueError("attn_tree takes 1 to %d drafted tokens a sequence, named by as many bits of a mask (max_nodes %d, masks of %d words)"
+                         % (MAX_TREE_NODES, max_nodes, words))
+    if n_splits < 1 or window < 0:
+        raise ValueError("attn_tree: n_splits %d, window %d" % (n_splits, window))
+    p_w = _need(partial, "partial", torch.float32)
+    need = attn_tree_workspace_floats(T, n_heads, head_dim, n_splits)
+    if partial.numel() < need:
+        raise ValueError("attn_tree workspace too small: %d floats, %d needed" % (partial.numel(), need))
+    library.check(library.lib().yalm_attn_tree(
+        p_q, p_kp, p_vp, p_bt, stride, n_slots, ring_pages, p_ss, _need(seq_len, "seq_len", torch.int32, (B,)),
+        _need(cu_nodes, "cu_nodes", torch.int32, (B + 1,)), p_m, words, _opt(positions, "positions", torch.int32, (T,)),
+        _need(out, "out", dt, width), p_w, T, B, n_heads, n_kv_heads, head_dim, int(window), int(n_splits), int(max_nodes), n_pages,
+        _layout(layout, head_dim), dtype_code(dt), 1 if FORCE_SIMPLE else 0, _opt(step_max_len, "step_max_len", torch.int32, (1,)), _stream()),
+        "attn_tree")
+    return out
+
+
 MAX_SINKS = 16
 
 
@@ -1894,6 +1951,77 @@ def token_prob(logits, index, out):
                                                 _need(index, "index", torch.int32, (R,)),
                                                 _need(out, "out", torch.float32, (R,)), R, V, _stream()), "token_prob")
     return out
+
+
+def sample_filtered_workspace(R, V):
+    """The int32 elements of sample_filtered's workspace (0: it takes none for these sizes)."""
+    return 0
+
+
+def sample_filtered(logits, u, out, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, workspace=None):
+    """One token for each row of logits (float32 [R, V]) under the row's own settings, float32 [R] on the device (top_k int32), each
+    optional: temperature (0: the first of the greatest), top_k (0: off), top_p (1: off), min_p (0: off).  With w = exp((l - max) /
+    temperature), tokens in the order of falling logits and rising indices: the first top_k, of those the shortest prefix that holds
+    top_p of their weight, of those the ones with w >= min_p; out[r] (int32) is the first of them, in the order of the indices, at which their
+    running sum reaches u[r] times its total (u in [0, 1)), prob[r] (float32, optional) its share of the total.  No number (NaN) is never drawn;
+    a row without a logit above -infinity gives -1 and 0."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+        raise ValueError("logits: float32 [rows, vocabulary] are expected")
+    R, V = logits.shape
+    if V < 1:
+        raise ValueError("sample_filtered needs a vocabulary")
+    n = (R,)
+    library.check(library.lib().yalm_sample_filtered(
+        _need(logits, "logits", torch.float32), _need(u, "u", torch.float32, n), _opt(temperature, "temperature", torch.float32, n),
+        _opt(top_k, "top_k", torch.int32, n), _opt(top_p, "top_p", torch.float32, n), _opt(min_p, "min_p", torch.float32, n),
+        _need(out, "out", torch.int32, n), _opt(prob, "prob", torch.float32, n), R, V, _stream()), "sample_filtered")
+    return out
+
+
+def copy_pages(k_pages, v_pages, src, dst):
+    """Page src[i] of every line of k_pages and v_pages ([lines, pages, ...], any type and shape of a page; v_pages may be None) to page
+    dst[i] (int32 [n] each, on the device).  No page may be the source of one pair and the destination of another; of several copies to one
+    page the last one stands, and a number that is no page is passed over."""
+    p_k = _need(k_pages, "k_pages")
+    p_v = None
+    if k_pages.dim() < 2:
+        raise ValueError("k_pages: [lines, pages, ...] is expected, got %s" % list(k_pages.shape))
+    if v_pages is not None:
+        p_v = _need(v_pages, "v_pages", k_pages.dtype)
+        if v_pages.shape[:2] != k_pages.shape[:2] or v_pages.numel() != k_pages.numel():
+            raise ValueError("v_pages %s are not the pages of k_pages %s" % (list(v_pages.shape), list(k_pages.shape)))
+    lines, pages = k_pages.shape[:2]
+    p_src = _need(src, "src", torch.int32, (None,))
+    p_dst = _need(dst, "dst", torch.int32, src.shape)
+    if k_pages.numel() == 0:
+        return
+    block = k_pages.numel() // (lines * pages) * k_pages.element_size()
+    library.check(library.lib().yalm_copy_blocks(p_k, p_v, lines, pages, block, p_src, p_dst, src.shape[0], _stream()), "copy_pages")
+
+
+def compact_lines(k_pages, v_pages, block_table, ring_pages, seq_slot, seq_start, cu_keep, keep, max_keep, layout=None):
+    """Moves kept tokens of the cache together: for sequence b (slot seq_slot[b], negative: none) the keys and values at the positions
+    seq_start[b] + keep[i], i from cu_keep[b] to cu_keep[b + 1] (at most max_keep of them), to seq_start[b], seq_start[b] + 1, ..., in every
+    line of k_pages [lines, pages, kv heads, PAGE, head_dim] and v_pages [lines, pages, kv heads, head_dim, PAGE].  keep ascends within a
+    sequence, so that no token is written over before it has moved; what stands behind the moved ones stays as it is.  All int32 on the device."""
+    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 5:
+        raise ValueError("k_pages: [lines, pages, kv heads, PAGE, head_dim] is expected")
+    dt = k_pages.dtype
+    L, n_pages, H, _, hd = k_pages.shape
+    p_k = _need(k_pages, "k_pages", dt, (L, n_pages, H, PAGE, hd))
+    p_v = _need(v_pages, "v_pages", dt, (L, n_pages, H, hd, PAGE))
+    p_t = _need(block_table, "block_table", torch.int32, (None, None))
+    n_slots, stride = block_table.shape
+    if ring_pages <= 0 or ring_pages > stride:
+        raise ValueError("ring_pages %d does not fit the block table (%d columns)" % (ring_pages, stride))
+    p_s = _need(seq_slot, "seq_slot", torch.int32, (None,))
+    B = seq_slot.shape[0]
+    if max_keep < 0:
+        raise ValueError("max_keep %d is negative" % max_keep)
+    library.check(library.lib().yalm_compact_lines(
+        p_k, p_v, p_t, stride, n_slots, ring_pages, p_s, _need(seq_start, "seq_start", torch.int32, (B,)),
+        _need(cu_keep, "cu_keep", torch.int32, (B + 1,)), _need(keep, "keep", torch.int32, (None,)), B, keep.shape[0], int(max_keep), L,
+        n_pages, H, hd, _layout(layout, hd), dtype_code(dt), _stream()), "compact_lines")
 
 
 def probe_read(src, workgroups=2048):

@@ -57,6 +57,10 @@ _SIGNATURES = {
     "yalm_attn_decode_static": (_I, [_P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "yalm_argmax": (_I, [_P, _P, _I, _I, _P]),
     "yalm_sample": (_I, [_P, _P, _F, _P, _I, _I, _P]),
+    "yalm_attn_tree": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
+    "yalm_sample_filtered": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
+    "yalm_copy_blocks": (_I, [_P, _P, _I, _I, ctypes.c_long, _P, _P, _I, _P]),
+    "yalm_compact_lines": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "yalm_token_prob": (_I, [_P, _P, _P, _I, _I, _P]),
     "yalm_gemm_add_emit": (_I, [_P, _P, _P, _P, ctypes.c_long, _I, _I, _I, _P, _P, _P, _P]),
     "yalm_gemm_add_emit_parts": (_I, [_I]),
@@ -118,7 +122,7 @@ _SIGNATURES = {
     "yalm_probe_mfma": (_I, [_I, _I, _I, _P, _P, _P]),
 }
 
-ABI_VERSION = 46
+ABI_VERSION = 47
 
 
 class KernelError(RuntimeError):
