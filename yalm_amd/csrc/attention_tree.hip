@@ -10,6 +10,9 @@
 #include "attention_tree.h"
 #include "yalm_hip.h"
 
+int yalm_attn_tree_bf16_mfma(const TreeArgs& a, hipStream_t stream);       // attention_tree_bf16.hip, attention_tree_f32.hip
+int yalm_attn_tree_f32_mfma(const TreeArgs& a, hipStream_t stream);
+
 namespace {
 
 // the last sequence whose first row is not behind r
@@ -86,6 +89,41 @@ __global__ __launch_bounds__(WAVE) void attn_tree_simple_kernel(TreeArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// The splits' parts [T, n_heads, n_splits, hd + 2] = (sum[hd], maximum as an exponent of 2, denominator), merged in one order: a
+// wave a (row, head).
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void attn_tree_merge_kernel(TreeArgs a) {
+  const int lane = threadIdx.x % WAVE, hd = a.head_dim, n = a.n_splits, stride = hd + 2;
+  const long head = (long)blockIdx.x * (256 / WAVE) + threadIdx.x / WAVE;
+  const int r = (int)(head / a.n_heads);
+  if (r >= min(a.cu_nodes[a.B], a.T)) return;
+  if (r - a.cu_nodes[sequence_of(a.cu_nodes, a.B, r)] >= a.max_nodes) return;
+  const float* part = a.partial + head * (long)n * stride;
+  float m = -FLT_MAX;
+  for (int s = lane; s < n; s += WAVE) m = fmaxf(m, part[(long)s * stride + hd]);
+  m = wave_max(m);
+  float l = 0.f;
+  for (int s = lane; s < n; s += WAVE) l = fmaf(part[(long)s * stride + hd + 1], __builtin_amdgcn_exp2f(part[(long)s * stride + hd] - m), l);
+  l = wave_sum(l);
+  const float inv = l > 0.f ? 1.0f / l : l == l ? 0.f : l;
+  T* out = (T*)a.out + head * hd;
+  for (int e = 2 * lane; e < hd; e += 2 * WAVE) {
+    float x = 0.f, y = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float* p = part + (long)s * stride;
+      const float f = __builtin_amdgcn_exp2f(p[hd] - m);
+      const float2 v = *reinterpret_cast<const float2*>(p + e);
+      x = fmaf(v.x, f, x);
+      y = fmaf(v.y, f, y);
+    }
+    out[e] = from_f32<T>(x * inv);
+    out[e + 1] = from_f32<T>(y * inv);
+  }
+}
+
 }  // namespace
 
 extern "C" int yalm_attn_tree(const void* q, const void* k_pages, const void* v_pages, const int* block_table, int table_stride,
@@ -101,11 +139,22 @@ extern "C" int yalm_attn_tree(const void* q, const void* k_pages, const void* v_
   const TreeArgs a = {q, k_pages, v_pages, block_table, table_stride, n_slots, ring_pages, seq_slot, seq_len, cu_nodes,
                       (const unsigned long long*)mask, mask_words, positions, out, partial, T, B, n_heads, n_kv_heads, head_dim, window,
                       n_splits, max_nodes, n_pages, page_layout, step_max_len};
-  if (dtype == YALM_F32)
-    attn_tree_simple_kernel<float><<<dim3(T, n_heads), WAVE, 0, stream>>>(a);
-  else if (dtype == YALM_BF16)
-    attn_tree_simple_kernel<bf16><<<dim3(T, n_heads), WAVE, 0, stream>>>(a);
-  else
-    return YALM_ERR_DTYPE;
+  if (dtype != YALM_F32 && dtype != YALM_BF16) return YALM_ERR_DTYPE;
+  // The matrix cores' kernels load and store 16 bytes a lane, from pages as the cache keeps them.
+  const uintptr_t at = (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (n_splits > 1 ? (uintptr_t)partial : 0);
+  const bool cores = !force_simple && head_dim % 16 == 0 && head_dim <= 128 && (at & 15) == 0 &&
+                     (page_layout == YALM_PAGE_BLOCKS) == (head_dim % 32 == 0);
+  if (!cores) {
+    if (dtype == YALM_F32) attn_tree_simple_kernel<float><<<dim3(T, n_heads), WAVE, 0, stream>>>(a);
+    else attn_tree_simple_kernel<bf16><<<dim3(T, n_heads), WAVE, 0, stream>>>(a);
+    return launch_status();
+  }
+  if (n_splits > 1 && partial == nullptr) return YALM_ERR_ARG;
+  const int rc = dtype == YALM_F32 ? yalm_attn_tree_f32_mfma(a, stream) : yalm_attn_tree_bf16_mfma(a, stream);
+  if (rc != YALM_OK || n_splits == 1) return rc;
+  const long groups = ((long)T * n_heads + 3) / 4;
+  if (groups > 0x7FFFFFFFl) return YALM_ERR_ARG;
+  if (dtype == YALM_F32) attn_tree_merge_kernel<float><<<(unsigned)groups, 256, 0, stream>>>(a);
+  else attn_tree_merge_kernel<bf16><<<(unsigned)groups, 256, 0, stream>>>(a);
   return launch_status();
 }

@@ -885,8 +885,22 @@ MAX_TREE_NODES = 256             # drafted tokens of a sequence that attn_tree t
 
 
 def attn_tree_splits(n_seqs, max_nodes, max_len, n_heads, n_kv_heads, head_dim, dtype, window=0):
-    """Into how many pieces attn_tree should cut the keys of a sequence."""
-    return 1
+    """Into how many pieces attn_tree should cut the keys of a sequence, so that its workgroups fill the chip: of steps of n_seqs sequences
+    of up to max_len tokens, the drafted ones (up to max_nodes) among them."""
+    if head_dim % 16 or head_dim > 128 or FORCE_SIMPLE:
+        return 1
+    cols = max_nodes * (n_heads // n_kv_heads)
+    if dtype == torch.float32:
+        tile, resident = (32 if cols > 16 and head_dim <= 96 else 16), 256
+    elif cols > 32 and head_dim % 32 == 0:
+        tile, resident = (128 if cols > 64 else 64), 256
+    else:
+        tile, resident = (32, 256) if cols > 16 else (16, 512)
+    pages = (max_len + PAGE - 1) // PAGE
+    if window:
+        pages = min(pages, (window + max_nodes + PAGE - 1) // PAGE + 1)
+    per = max(1, n_seqs * n_kv_heads * ((cols + tile - 1) // tile))
+    return max(1, min(resident // per, (pages + 3) // 4))
 
 
 def attn_tree_workspace_floats(T, n_heads, head_dim, n_splits):
