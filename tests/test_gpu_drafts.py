@@ -54,11 +54,14 @@ def draw_rows(logits, u, T, k, p, mp):
     out = torch.full((n,), -7, dtype=torch.int32, device=DEV)
     prob = torch.full((n,), float("nan"), device=DEV)
     x = logits.to(DEV)
-    ws = torch.zeros(K().sample_filtered_workspace(*x.shape), dtype=torch.int32, device=DEV)
-    K().sample_filtered(x, dev(u, torch.float32), out, temperature=dev(T, torch.float32), top_k=dev(k, torch.int32),
-                        top_p=dev(p, torch.float32), min_p=dev(mp, torch.float32), prob=prob, workspace=ws)
-    assert not ws.any()
-    return out, prob
+    args = dict(temperature=dev(T, torch.float32), top_k=dev(k, torch.int32), top_p=dev(p, torch.float32), min_p=dev(mp, torch.float32))
+    # a row a workgroup, and rows over several of them through a workspace that holds anything
+    K().sample_filtered(x, dev(u, torch.float32), out, prob=prob, **args)
+    ws = torch.randint(-2 ** 31, 2 ** 31 - 1, (K().sample_filtered_workspace(*x.shape),), dtype=torch.int32, device=DEV)
+    out2, prob2 = torch.full_like(out, -9), torch.full_like(prob, float("nan"))
+    K().sample_filtered(x, dev(u, torch.float32), out2, prob=prob2, workspace=ws, **args)
+    assert torch.equal(out, out2) and torch.equal(prob, prob2)
+    return out2, prob2
 
 
 SETTINGS = [(1.0, 0, 1.0, 0.0), (0.8, 40, 0.95, 0.0), (1.3, 0, 0.9, 0.0), (0.5, 0, 1.0, 0.1), (1.0, 1, 1.0, 0.0), (0.7, 300, 0.5, 0.02),

@@ -329,9 +329,11 @@ int yalm_token_prob(const float* logits, const int* index, float* prob, int R, i
 // more: all of K; at least one), M those of P with w >= min_p[r]; out[r] = the first token of M in the order of the indices at which M's
 // running sum reaches u[r] times its total, prob[r] (may be null) its share of that total.  temperature[r] <= 0: the first of the
 // greatest, probability 1.  No number (NaN) is never drawn; a row without a logit above -infinity gives -1 and 0.  The settings are float32 (top_k
-// int32) [R] on the device; a null pointer stands for temperature 1 or a filter that is off.
+// int32) [R] on the device; a null pointer stands for temperature 1 or a filter that is off.  workspace (may be null, then a row is one
+// workgroup's): yalm_sample_filtered_workspace bytes on 16 bytes, of any content.
 int yalm_sample_filtered(const float* logits, const float* u, const float* temperature, const int* top_k, const float* top_p,
-                         const float* min_p, int* out, float* prob, int R, int V, hipStream_t stream);
+                         const float* min_p, int* out, float* prob, void* workspace, int R, int V, hipStream_t stream);
+long yalm_sample_filtered_workspace(int R, int V);
 
 // Pages that move (cache_pages.hip).  yalm_copy_blocks: block src[i] of each of the n_lines lines of a (and of b, may be null), lines of
 // n_blocks blocks of block_bytes each, to block dst[i]; no block is a source and another pair's destination; of several copies to

@@ -1969,7 +1969,7 @@ def token_prob(logits, index, out):
 
 def sample_filtered_workspace(R, V):
     """The int32 elements of sample_filtered's workspace (0: it takes none for these sizes)."""
-    return 0
+    return library.lib().yalm_sample_filtered_workspace(R, V) // 4
 
 
 def sample_filtered(logits, u, out, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, workspace=None):
@@ -1978,17 +1978,25 @@ def sample_filtered(logits, u, out, temperature=None, top_k=None, top_p=None, mi
     temperature), tokens in the order of falling logits and rising indices: the first top_k, of those the shortest prefix that holds
     top_p of their weight, of those the ones with w >= min_p; out[r] (int32) is the first of them, in the order of the indices, at which their
     running sum reaches u[r] times its total (u in [0, 1)), prob[r] (float32, optional) its share of the total.  No number (NaN) is never drawn;
-    a row without a logit above -infinity gives -1 and 0."""
+    a row without a logit above -infinity gives -1 and 0.  workspace (int32, at least sample_filtered_workspace elements of any content, not shared
+    with a call that may run at the same time): with it a row is spread over several workgroups; the results are the same."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise ValueError("logits: float32 [rows, vocabulary] are expected")
     R, V = logits.shape
     if V < 1:
         raise ValueError("sample_filtered needs a vocabulary")
     n = (R,)
+    p_ws = None
+    if workspace is not None:
+        p_ws = _need(workspace, "workspace", torch.int32)
+        if workspace.numel() < sample_filtered_workspace(R, V):
+            raise ValueError("sample_filtered workspace too small: %d elements, %d needed" % (workspace.numel(), sample_filtered_workspace(R, V)))
+        if p_ws % 16 or workspace.numel() == 0:
+            p_ws = None                       # a part of a buffer that the kernels' 16-byte loads cannot take: as without one
     library.check(library.lib().yalm_sample_filtered(
         _need(logits, "logits", torch.float32), _need(u, "u", torch.float32, n), _opt(temperature, "temperature", torch.float32, n),
         _opt(top_k, "top_k", torch.int32, n), _opt(top_p, "top_p", torch.float32, n), _opt(min_p, "min_p", torch.float32, n),
-        _need(out, "out", torch.int32, n), _opt(prob, "prob", torch.float32, n), R, V, _stream()), "sample_filtered")
+        _need(out, "out", torch.int32, n), _opt(prob, "prob", torch.float32, n), p_ws, R, V, _stream()), "sample_filtered")
     return out
 
 

@@ -58,7 +58,8 @@ _SIGNATURES = {
     "yalm_argmax": (_I, [_P, _P, _I, _I, _P]),
     "yalm_sample": (_I, [_P, _P, _F, _P, _I, _I, _P]),
     "yalm_attn_tree": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
-    "yalm_sample_filtered": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
+    "yalm_sample_filtered": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
+    "yalm_sample_filtered_workspace": (ctypes.c_long, [_I, _I]),
     "yalm_copy_blocks": (_I, [_P, _P, _I, _I, ctypes.c_long, _P, _P, _I, _P]),
     "yalm_compact_lines": (_I, [_P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "yalm_token_prob": (_I, [_P, _P, _P, _I, _I, _P]),
