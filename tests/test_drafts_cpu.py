@@ -35,3 +35,125 @@ def test_workspace_sizes():
     assert kernels.attn_tree_workspace_floats(7, 4, 64, 1) == 0
     assert kernels.attn_tree_workspace_floats(7, 4, 64, 3) == 7 * 4 * 3 * 66
     assert kernels.sample_filtered_workspace(3, 32000) >= 0
+
+
+# ------------------------------------------------------------------------------------------------ pages that are shared
+def _cache(max_tokens=1024, window=0, n_slots=8, sinks=0, max_draft=0):
+    from yalm_amd.cache import CacheManager, KVRequest, StateRequest
+    req = {0: KVRequest(1, 4, window, sinks), 1: KVRequest(1, 4, window, sinks), 2: StateRequest((3,))}
+    return CacheManager(req, max_tokens, max_tokens, torch.float32, "cpu", n_slots=n_slots, max_draft=max_draft)
+
+
+def test_a_page_is_free_when_the_last_holder_gives_it_back():
+    from yalm_amd.cache import CacheError, PagePool
+    p = PagePool(2)
+    a = p.take()
+    p.share(a)
+    assert p.holders(a) == 2 and p.n_free == 1
+    p.give_back(a)
+    assert p.holders(a) == 1 and p.n_free == 1
+    p.give_back(a)
+    assert p.n_free == 2
+    for bad in (p.give_back, p.share):
+        with pytest.raises(CacheError):
+            bad(a)
+
+
+def test_forks_share_full_pages_and_copy_the_last_one():
+    c = _cache()
+    (s,) = c.acquire(1)
+    c.extend([s], [150])
+    g = c.kv_groups[0]
+    new, copies = c.fork(s, 2)
+    table = g.table_host
+    for t in new:
+        assert c.seq_len[t] == 150 and (table[t, :2] == table[s, :2]).all() and table[t, 2] != table[s, 2]
+    assert table[new[0], 2] != table[new[1], 2] and g.pool.holders(int(table[s, 0])) == 3 and g.pool.n_free == 16 - 5
+    (k, v, src, dst), (state, none, src_s, dst_s) = copies
+    assert k is g.k_pages and v is g.v_pages and src == [int(table[s, 2])] * 2 and dst == [int(table[t, 2]) for t in new]
+    assert state is c.state_groups[0].data and none is None and src_s == [s, s] and dst_s == new
+    assert torch.equal(g.table, torch.from_numpy(table))
+    c.extend([s] + new, [64, 1, 43])                   # each goes on in pages of its own
+    assert len({int(table[t, 2]) for t in [s] + new}) == 3 and int(table[s, 3]) != int(table[new[1], 3]) >= 0
+    c.release([s])
+    assert g.pool.holders(int(table[new[0], 0])) == 2
+    c.release(new)
+    assert g.pool.n_free == g.n_pages and c.slots.n_free == 8
+    (t,) = c.acquire(1)
+    c.extend([t], [128])                               # a prompt that ends with its page: nothing to copy but the state
+    new, copies = c.fork(t, 1)
+    assert len(copies) == 1 and g.pool.n_free == 16 - 2
+
+
+def test_forks_of_windows_and_sinks_are_copies_and_what_does_not_fit_changes_nothing():
+    from yalm_amd.cache import CacheError, CacheFull
+    c = _cache(window=100, sinks=2)
+    (s,) = c.acquire(1)
+    c.extend([s], [500])
+    g = c.kv_groups[0]
+    new, copies = c.fork(s, 1)
+    assert g.ring_pages == 3 and len(copies) == 3 and copies[0][2] == [int(p) for p in g.table_host[s]] and copies[1][0] is g.sink_k
+    assert g.pool.n_free == 16 - 6
+    free = (g.pool.n_free, c.slots.n_free, g.table_host.copy())
+    with pytest.raises(CacheFull, match="pages"):
+        c.fork(s, 4)
+    with pytest.raises(CacheFull, match="slots"):
+        c.fork(s, 9)
+    for bad in ((7, 1), (s, -1)):
+        with pytest.raises(CacheError):
+            c.fork(*bad)
+    assert (g.pool.n_free, c.slots.n_free) == free[:2] and (g.table_host == free[2]).all()
+    assert c.fork(s, 0) == ([], [])
+
+
+@pytest.mark.parametrize("window", [0, 100])
+def test_cut_sequences_give_back_their_pages(window):
+    from yalm_amd.cache import CacheError
+    c = _cache(window=window, max_draft=70)
+    g = c.kv_groups[0]
+    assert g.ring_pages == (16 if not window else (100 + 69 + 63) // 64 + 1)
+    (s,) = c.acquire(1)
+    for base, more, to in ((60, 70, 61), (61, 3, 64), (64, 64, 64), (64, 65, 65), (65, 63, 128), (300, 70, 310)):
+        c.extend([s], [base - c.seq_len[s]] if base > c.seq_len[s] else [0]) if base != c.seq_len[s] else None
+        c.extend([s], [more])
+        c.cut([s], [to])
+        held = [int(p) for p in g.table_host[s] if p >= 0]
+        assert c.seq_len[s] == to and len(held) == len(set(held)) and g.pool.n_free == 16 - len(held)
+        assert len(held) == min((to + 63) // 64, g.ring_pages) or window
+    for bad in (-1, 311):
+        with pytest.raises(CacheError):
+            c.cut([s], [bad])
+    c.release([s])
+    assert g.pool.n_free == 16
+
+
+# ------------------------------------------------------------------------------------------------ guesses
+def test_guesses_from_a_text_itself():
+    from yalm_amd.drafting import _shallow, accept, lookup_tree
+    text = [5, 6, 7, 8, 9, 1, 5, 6, 7, 2, 3, 5, 6]
+    tokens, parents = lookup_tree(text, 7)
+    assert tokens == [6, 7, 2, 3, 8, 9] and parents == [-1, 0, 1, 2, 1, 4]        # the later place first, the common 7 once
+    assert lookup_tree([4], 5) == ([4], [-1]) and lookup_tree([1, 2, 3], 5) == ([3], [-1])
+    assert lookup_tree(text, 1) == ([6], [-1])
+    for n in range(1, 30):
+        tokens, parents = lookup_tree([1, 2] * 20, n)
+        assert len(tokens) <= n and parents[0] == -1 and all(p < j for j, p in enumerate(parents))
+    tokens, parents = [6, 7, 2, 3, 8, 9], [-1, 0, 1, 2, 1, 4]
+    assert accept(tokens, parents, [7, 8, 0, 0, 9, 4]) == ([0, 1, 4, 5], [7, 8, 9, 4])
+    assert accept(tokens, parents, [1, 8, 0, 0, 9, 4]) == ([0], [1])
+    assert accept(tokens, parents, [7, 2, 3, 6, 0, 0]) == ([0, 1, 2, 3], [7, 2, 3, 6])
+    assert _shallow(tokens, parents, 2) == ([6, 7], [-1, 0], [0, 1])
+    assert _shallow(tokens, parents, 3) == ([6, 7, 2, 8], [-1, 0, 1, 1], [0, 1, 2, 2])
+    assert _shallow(tokens, parents, 1) == ([6], [-1], [0])
+
+
+def test_command_line_settings():
+    from yalm_amd.cli import parse_args
+    a = parse_args(["folder", "--tokens", "1,2", "--top-k", "40", "--top-p", "0.9", "--min-p", "0.05", "--samples", "3"])
+    assert (a["top_k"], a["top_p"], a["min_p"], a["samples"], a["draft"]) == (40, 0.9, 0.05, 3, 0)
+    assert parse_args(["folder", "--tokens", "1,2", "--draft", "8"])["draft"] == 8
+    d = parse_args(["folder", "--tokens", "1,2"])
+    assert (d["top_k"], d["top_p"], d["min_p"], d["samples"], d["draft"]) == (0, 1.0, 0.0, 1, 0)
+    for bad in (["--top-k", "-1"], ["--top-p", "1.2"], ["--min-p", "-0.1"], ["--samples", "0"], ["--draft", "-2"], ["--draft", "2", "--samples", "2"]):
+        with pytest.raises(SystemExit):
+            parse_args(["folder", "--tokens", "1,2"] + bad)

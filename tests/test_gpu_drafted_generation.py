@@ -1,0 +1,254 @@
+"""Drafted tokens, forked sequences and filtered sampling through the engine and the generation loops: a tree's logits against
+the plain implementation on each node's own text, what is kept of it against the text without drafts, and the loops' tokens against the
+ones that generate() gives without them."""
+import numpy as np
+import pytest
+import torch
+
+import bovozen_configs
+import gemepel_configs
+import helpers
+import tiny_configs
+import zebivik_configs
+from plain import reference_model as R
+from test_gpu_drafts import sample_reference
+
+pytestmark = pytest.mark.gpu
+NAMES = ["tiny_llama", "tiny_mistral", "tiny_llama3", "tiny_wide_heads"]
+
+
+@pytest.fixture(scope="module")
+def folders(tmp_path_factory):
+    tmp = tmp_path_factory.mktemp("draft_models")
+    return {name: helpers.make_folder(tmp, name, tiny_configs.ALL[name], seed=8) for name in NAMES}
+
+
+def engine_of(folders, name, dtype, **kw):
+    from yalm_amd import Engine, Model
+    return Engine(Model.from_folder(folders[name], dtype=dtype, device="cuda:0"), **{"max_tokens": 1024, "max_batch": 6, "max_draft": 20, **kw})
+
+
+def tree(n, seed):
+    rng = np.random.default_rng(seed)
+    return [-1] + [int(rng.integers(max(0, j - 4), j)) for j in range(1, n)]
+
+
+def path_to(parents, j):
+    out = []
+    while j >= 0:
+        out.append(j)
+        j = parents[j]
+    return out[::-1]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", NAMES)
+def test_a_tree_s_logits_and_what_is_kept_of_it(folders, name, dtype):
+    """Trees of several sizes behind prompts of several lengths (past the window of the Mistral one, over a page's end), three rounds of
+    them, a plain step behind each: every logit is that of the node's own text."""
+    engine = engine_of(folders, name, helpers.torch_dtype(dtype))
+    cfg = tiny_configs.ALL[name]
+    V, limit = cfg["vocab_size"], engine.n_positions
+    rng = np.random.default_rng(3)
+    texts = [rng.integers(0, V, n).tolist() for n in (1, 17, min(limit - 30, 59))]
+    slots = engine.start(3)
+    engine.step(slots, texts)
+
+    def check(got, text, what):
+        helpers.check_logits(got[None], helpers.plain_logits(folders[name], tuple(text), dtype)[-1:], dtype, what)
+
+    for turn, sizes in enumerate([(5, 1, 12), (2, 9, 3), (1, 6, 4)]):
+        trees = [tree(n, 10 * turn + n) for n in sizes]
+        tokens = [rng.integers(0, V, n).tolist() for n in sizes]
+        logits = engine.draft_step(slots, tokens, trees).float().cpu().numpy()
+        row = 0
+        paths = []
+        for i, (toks, up) in enumerate(zip(tokens, trees)):
+            for j in range(len(toks)):
+                check(logits[row + j], texts[i] + [toks[k] for k in path_to(up, j)], "turn %d, sequence %d, node %d" % (turn, i, j))
+            row += len(toks)
+            paths.append(path_to(up, int(rng.integers(0, len(toks)))) if (turn, i) != (1, 0) else [])
+        engine.keep(slots, paths)
+        for i, path in enumerate(paths):
+            texts[i] = texts[i] + [tokens[i][j] for j in path]
+            assert engine.length(slots[i]) == len(texts[i])
+        more = [[int(t)] for t in rng.integers(0, V, 3)]
+        got = engine.step(slots, more).float().cpu().numpy()
+        for i in range(3):
+            texts[i] = texts[i] + more[i]
+            check(got[i], texts[i], "the step behind turn %d, sequence %d" % (turn, i))
+    engine.release(slots)
+    assert all(g.pool.n_free == g.n_pages for g in engine.cache.kv_groups)
+
+
+@pytest.mark.parametrize("filters", [{}, {"temperature": 0.9}, {"temperature": 0.8, "top_k": 20, "top_p": 0.9}, {"temperature": 1.1, "min_p": 0.05}])
+@pytest.mark.parametrize("name", ["tiny_llama", "tiny_mistral", "tiny_llama3"])
+def test_drafted_generation_gives_the_tokens_of_generate(folders, name, filters):
+    """float32: the same tokens with trees of guesses as without, guessed from the text, by an oracle and by one that is always wrong;
+    stop tokens end a request where they stand; the cache is whole again."""
+    from yalm_amd import GenerationStats, generate, generate_drafted
+    engine = engine_of(folders, name, torch.float32)
+    V = tiny_configs.ALL[name]["vocab_size"]
+    rng = np.random.default_rng(5)
+    prompts = [(rng.integers(0, V, 4).tolist() * 6)[:n] for n in (2, 9, 21)] + [rng.integers(0, V, 5).tolist() for _ in range(4)]
+    args = dict(max_new_tokens=24, seed=11, stop_ids=[], **{"temperature": 0.0, **filters})
+    want = generate(engine, prompts, **args)
+    assert generate_drafted(engine, prompts, **args) == want
+
+    def oracle(history, n):
+        which = next(i for i, p in enumerate(prompts) if history[:len(p)] == p and want[i][:len(history) - len(p)] == history[len(p):])
+        ahead = (prompts[which] + want[which])[len(history) - 1:][:n]
+        return ahead, list(range(-1, len(ahead) - 1))
+
+    stats = GenerationStats()
+    assert generate_drafted(engine, prompts, guess=oracle, max_nodes=5, stats=stats, batch_size=1, **args) == want
+    assert stats.decode_steps < stats.new_tokens / 2 and stats.new_tokens == sum(map(len, want))
+    wrong = lambda history, n: ([history[-1]] + [0] * (n - 1), [-1] + [0] * (n - 1))  # noqa: E731
+    assert generate_drafted(engine, prompts, guess=wrong, max_nodes=3, **args) == want
+    stop = want[1][5]
+    cut = generate(engine, prompts, **{**args, "stop_ids": [stop]})
+    assert generate_drafted(engine, prompts, guess=oracle, max_nodes=7, **{**args, "stop_ids": [stop]}) == cut
+    assert not engine.cache.slots.held and all(g.pool.n_free == g.n_pages for g in engine.cache.kv_groups)
+
+
+def test_drafted_generation_up_to_the_end_of_the_context(folders):
+    from yalm_amd import generate, generate_drafted
+    engine = engine_of(folders, "tiny_llama", torch.float32, max_tokens=128, max_batch=1)
+    prompt = [3, 9, 4] * 30
+    want = generate(engine, [prompt], max_new_tokens=100, stop_ids=[])
+    assert len(want[0]) == engine.n_positions - len(prompt)
+    assert generate_drafted(engine, [prompt], max_new_tokens=100, stop_ids=[], max_nodes=16) == want
+
+
+@pytest.mark.parametrize("name", ["tiny_llama", "tiny_mistral"])
+def test_filters_in_the_generation_loop(folders, name):
+    """Tokens are the definition's picks from the plain implementation's logits."""
+    from yalm_amd import generate
+    from yalm_amd.sampling import uniform
+    engine = engine_of(folders, name, torch.float32)
+    prompt = [7, 100, 31, 5]
+    got = generate(engine, [prompt], max_new_tokens=12, temperature=0.7, top_k=30, top_p=0.8, min_p=0.01, seed=5, stop_ids=[])[0]
+    assert generate(engine, [prompt], max_new_tokens=12, temperature=0.7, top_k=30, top_p=0.8, min_p=0.01, seed=5, stop_ids=[], ahead=False)[0] == got
+    cfg, w = R.read_folder(folders[name])
+    agree = 0
+    for step in range(12):
+        logits = R.forward(w, cfg, prompt + got[:step])[-1].float().numpy()
+        agree += sample_reference(logits, uniform(5, 0, step), 0.7, 30, 0.8, 0.01)[0] == got[step]
+    assert agree >= 11                                         # a number may lie within the logits' rounding of a border
+    greedy = generate(engine, [prompt], max_new_tokens=6, stop_ids=[])
+    assert generate(engine, [prompt], max_new_tokens=6, top_k=5, top_p=0.5, stop_ids=[]) == greedy
+    assert generate(engine, [prompt], max_new_tokens=6, temperature=2.0, top_k=1, stop_ids=[]) == greedy
+
+
+def test_settings_for_each_row_and_their_refusals():
+    from yalm_amd import Sampler
+    logits = torch.randn((4, 500), generator=torch.Generator().manual_seed(1)).to("cuda:0")
+    s = Sampler(3)
+    one = [s.sample(logits[i:i + 1], t, [i], [2], top_k=k, top_p=p, min_p=m)[0]
+           for i, (t, k, p, m) in enumerate([(0.0, 3, 0.5, 0.0), (0.7, 0, 0.9, 0.0), (1.0, 9, 1.0, 0.1), (1.2, 0, 1.0, 0.0)])]
+    every = s.sample(logits, [0.0, 0.7, 1.0, 1.2], range(4), [2] * 4, top_k=[3, 0, 9, 0], top_p=[0.5, 0.9, 1.0, 1.0], min_p=[0.0, 0.0, 0.1, 0.0])
+    assert every == one and one[0] == int(logits[0].argmax())
+    for bad in ({"top_p": 1.5}, {"min_p": -0.1}, {"top_k": -1}, {"top_k": [1, 2]}, {"top_p": float("nan")}):
+        with pytest.raises(ValueError):
+            s.sample(logits, 0.7, range(4), [0] * 4, **bad)
+    with pytest.raises(ValueError):
+        s.sample(logits, -1.0, range(4), [0] * 4, top_k=3)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", NAMES)
+def test_several_answers_to_a_prompt(folders, name, dtype):
+    """samples=n gives what n requests of the same prompt give, each from its own number; forks and the sequence they came from then go
+    on independently."""
+    from yalm_amd import GenerationStats, generate
+    engine = engine_of(folders, name, helpers.torch_dtype(dtype), max_batch=7)
+    V = tiny_configs.ALL[name]["vocab_size"]
+    prompts = [np.random.default_rng(n).integers(0, V, n).tolist() for n in (3, 40, 8)]
+    stats = GenerationStats()
+    got = generate(engine, prompts, max_new_tokens=10, temperature=0.9, seed=4, stop_ids=[], samples=3, stats=stats)
+    assert len(got) == 9 and stats.new_tokens == 90 and stats.prompt_tokens < 3 * sum(map(len, prompts))
+    if dtype == "float32":
+        assert got == generate(engine, [p for p in prompts for _ in range(3)], max_new_tokens=10, temperature=0.9, seed=4, stop_ids=[])
+    assert not engine.cache.slots.held and all(g.pool.n_free == g.n_pages for g in engine.cache.kv_groups)
+
+
+CARRYING = {"zebivik": zebivik_configs, "gemepel": gemepel_configs, "bovozen": bovozen_configs}
+
+
+@pytest.mark.parametrize("design", sorted(CARRYING))
+def test_forks_of_designs_that_carry_state(design):
+    """A fork's logits are bit for bit those of the sequence it came from, and trees are refused."""
+    from yalm_amd import Engine, Model, StepError
+    cfg = next(v for k, v in vars(CARRYING[design]).items() if k.isupper() and isinstance(v, dict) and "layers" in v)
+    engine = Engine(Model.random(cfg, 3, dtype=torch.float32), max_tokens=1024, max_batch=4)
+    (s,) = engine.start(1)
+    engine.step([s], [[5, 9, 2, 7, 1, 3, 8]])
+    engine.step([s], [[4]])
+    new = engine.fork(s, 2)
+    for tok in (6, 1, 9):
+        logits = [engine.step([x], [[tok]]).clone() for x in [s] + new]
+        assert torch.equal(logits[0], logits[1]) and torch.equal(logits[0], logits[2])
+    a, b = (engine.step([x], [[t]]).clone() for x, t in zip(new, (2, 3)))
+    assert not torch.equal(a, b)
+    with pytest.raises(StepError, match="drafted"):
+        engine.draft_step([s], [[1, 2]])
+
+
+def test_refused_drafts(folders):
+    from yalm_amd import Engine, Model, StepError
+    engine = engine_of(folders, "tiny_mistral", torch.float32, max_draft=6)
+    a, b = engine.start(2)
+    with pytest.raises(StepError, match="after its prompt"):
+        engine.draft_step([a], [[1, 2]])
+    engine.step([a, b], [[1, 2, 3], [4]])
+    for tokens, parents, match in ([[1] * 7], None, "drafted tokens"), ([[]], None, "drafted tokens"), ([[1, 400]], None, "vocabulary"), \
+            ([[1, 2, 3]], [[-1, 0, 2]], "parent"), ([[1, 2]], [[-1]], "parent"), ([[1], [2]], None, "same length"):
+        with pytest.raises(StepError, match=match):
+            engine.draft_step([a], tokens, parents)
+    with pytest.raises(StepError, match="no drafted"):
+        engine.keep([a], [[0]])
+    engine.draft_step([a], [[1, 2, 3]], [[-1, 0, 0]])
+    for path in ([1], [0, 1, 2], [0, 3], [0, 0]):
+        with pytest.raises(StepError, match="path"):
+            engine.keep([a], [path])
+    for call in (lambda: engine.step([a], [[1]]), lambda: engine.draft_step([a], [[1]]), lambda: engine.fork(a, 1)):
+        with pytest.raises(StepError, match="drafted"):
+            call()
+    engine.step([b], [[1]])
+    with pytest.raises(StepError, match="one path"):
+        engine.keep([a, a], [[0], [0]])
+    engine.keep([a], [[0, 2]])
+    engine.step([a], [[1]])
+    engine.draft_step([a], [[1, 2]])
+    engine.release([a])                                        # a sequence may end with its drafts undecided
+    (c,) = engine.start(1)
+    engine.step([c], [[5, 6]])
+    assert Engine(engine.model, max_tokens=512).max_draft == 0
+    sinks = Engine(Model.from_folder(folders["tiny_llama"], dtype=torch.float32, device="cuda:0", context=20), max_tokens=512, max_draft=4)
+    (s,) = sinks.start(1)
+    sinks.step([s], [[1, 2, 3]])
+    with pytest.raises(StepError, match="sinks"):
+        sinks.draft_step([s], [[1, 2]])
+
+
+def test_the_command_line_samples_and_drafts(folders, capsys):
+    from yalm_amd import generate
+    from yalm_amd.cli import main
+    engine = engine_of(folders, "tiny_llama", torch.float32)
+    prompt = [1, 5, 17, 1, 5]
+    args = [folders["tiny_llama"], "--tokens", "1,5,17,1,5", "-n", "7", "--dtype", "float32", "--seed", "3"]
+
+    def run(*more):
+        main(args + list(more))
+        return capsys.readouterr().out
+
+    filters = dict(temperature=0.8, top_k=30, top_p=0.9, seed=3)
+    flags = ["-t", "0.8", "--top-k", "30", "--top-p", "0.9"]
+    stop = [2]
+    want = generate(engine, [prompt], max_new_tokens=7, stop_ids=stop, samples=2, **filters)
+    out = run(*flags, "--samples", "2")
+    assert all("[%d] %s\n" % (i, " ".join(map(str, w))) in out for i, w in enumerate(want))
+    want = generate(engine, [prompt], max_new_tokens=7, stop_ids=stop, **filters)[0]
+    assert " ".join(map(str, want)) in run(*flags, "--draft", "4")
+    with pytest.raises(SystemExit):
+        main(args + ["--draft", "4", "-T", "16"])

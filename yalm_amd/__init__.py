@@ -11,10 +11,11 @@ loop with sampling, hand-written HIP kernels, and trace replay.
 from . import parts  # noqa: F401  (registers the parts)
 from .config import config_from_dict, config_from_folder, register_architecture
 from .engine import Engine, Model, StepError
+from .drafting import generate_drafted
 from .generate import GenerationStats, generate
 from .parts import register_part
 from .sampling import Sampler
 from .weights import write_random_model
 
-__all__ = ["Engine", "Model", "StepError", "GenerationStats", "generate", "Sampler", "config_from_dict",
+__all__ = ["Engine", "Model", "StepError", "GenerationStats", "generate", "generate_drafted", "Sampler", "config_from_dict",
            "config_from_folder", "register_architecture", "register_part", "write_random_model"]

@@ -99,24 +99,36 @@ class SlotAllocator:
 
 
 class PagePool:
-    """Page numbers of one group."""
+    """Page numbers of one group.  A page may be held by several sequences (one that goes on from another's tokens shares the pages
+    that the tokens fill); it is free again when the last of them has given it back."""
 
     def __init__(self, n_pages):
         self.n_pages = n_pages
         self._free = list(range(n_pages - 1, -1, -1))
-        self._held = set()
+        self._held = {}                                # page -> who holds it
 
     def take(self):
         if not self._free:
             raise CacheFull("the cache has no free page left (%d pages)" % self.n_pages)
         p = self._free.pop()
-        self._held.add(p)
+        self._held[p] = 1
         return p
+
+    def share(self, page):
+        if page not in self._held:
+            raise CacheError("page %r is shared but not held" % (page,))
+        self._held[page] += 1
+
+    def holders(self, page):
+        return self._held.get(page, 0)
 
     def give_back(self, page):
         if page not in self._held:
             raise CacheError("page %r is given back but not held" % (page,))
-        self._held.remove(page)
+        if self._held[page] > 1:
+            self._held[page] -= 1
+            return
+        del self._held[page]
         self._free.append(page)
 
     @property
@@ -127,7 +139,7 @@ class PagePool:
 class KVGroup:
     """Pages and block table of the cache lines that share one KVRequest."""
 
-    def __init__(self, request, lines, n_pages, n_slots, max_seq_len, dtype, device):
+    def __init__(self, request, lines, n_pages, n_slots, max_seq_len, dtype, device, max_draft=0):
         self.request = request
         self.lines = list(lines)                       # cache line ids, in storage order
         self.line_index = {l: i for i, l in enumerate(self.lines)}
@@ -135,7 +147,8 @@ class KVGroup:
         self.window = request.window
         full_pages = max(1, pages_for(max_seq_len))
         if self.window > 0:
-            self.ring_pages = min(full_pages, pages_for(self.window) + 1)
+            # drafted tokens lie behind the ones that the first of them sees
+            self.ring_pages = min(full_pages, pages_for(self.window + max(max_draft - 1, 0)) + 1)
         else:
             self.ring_pages = full_pages
         self.n_pages = n_pages
@@ -199,6 +212,44 @@ class KVGroup:
                     self.table_host[slot, col] = self.pool.take()
                     self._dirty.add(slot)
 
+    def columns(self, length):
+        """The columns of the block table that a sequence of `length` tokens holds pages in."""
+        return min(pages_for(length), self.ring_pages)
+
+    def fork_pages(self, slot, length, new):
+        """The pages of a sequence of `length` tokens for the slots `new` that go on from it: full ones are shared, the one that they
+        will write on in, or with a window every one (the ring comes round to it), is theirs alone.  Returns the copies to make, (from,
+        to) a page."""
+        n = self.columns(length)
+        shared = 0 if self.window > 0 else length // PAGE
+        copies = []
+        for s in new:
+            for col in range(n):
+                page = int(self.table_host[slot, col])
+                if col < shared:
+                    self.pool.share(page)
+                else:
+                    to = self.pool.take()
+                    copies.append((page, to))
+                    page = to
+                self.table_host[s, col] = page
+            self._dirty.add(s)
+        return copies
+
+    def fork_needs(self, length, n):
+        """The pages that fork_pages takes for n slots."""
+        return n * (self.columns(length) - (0 if self.window > 0 else length // PAGE))
+
+    def cut(self, slot, old_len, new_len):
+        """Gives back the pages behind new_len of a sequence of old_len tokens (those of a ring stay: it keeps them all)."""
+        if self.window > 0 and pages_for(new_len) >= self.ring_pages:
+            return
+        row = self.table_host[slot]
+        for col in range(self.columns(new_len), self.columns(old_len)):
+            self.pool.give_back(int(row[col]))
+            row[col] = -1
+            self._dirty.add(slot)
+
     def free_slot(self, slot):
         row = self.table_host[slot]
         for col in range(self.ring_pages):
@@ -254,9 +305,10 @@ class CacheManager:
     requests: {cache line id: KVRequest | StateRequest | None, or {name: such a request, or such a dictionary}: a
     layer made of several members that keep something has the line (id, name) for each}
     max_tokens: the most tokens live sequences hold at any time, each sequence's
-    count rounded up to a multiple of PAGE."""
+    count rounded up to a multiple of PAGE.  max_draft: the most drafted tokens that a sequence goes on by at once (the rings
+    of windowed groups have room for them)."""
 
-    def __init__(self, requests, max_tokens, max_seq_len, dtype, device, n_slots=None):
+    def __init__(self, requests, max_tokens, max_seq_len, dtype, device, n_slots=None, max_draft=0):
         if max_tokens <= 0:
             raise CacheError("max_tokens must be positive")
         self.device = device
@@ -281,7 +333,7 @@ class CacheManager:
         self._group_of_line = {}
         for req, lines in by_request.items():
             if isinstance(req, KVRequest):
-                g = KVGroup(req, sorted(lines, key=_line_order), self.n_pages, self.n_slots, self.max_seq_len, dtype, device)
+                g = KVGroup(req, sorted(lines, key=_line_order), self.n_pages, self.n_slots, self.max_seq_len, dtype, device, max_draft)
                 self.kv_groups.append(g)
             elif isinstance(req, StateRequest):
                 g = StateGroup(req, sorted(lines, key=_line_order), self.n_slots, device)
@@ -344,6 +396,49 @@ class CacheManager:
         for s, nl in zip(slots, new_lens):
             seq_len[s] = nl
         return new_lens
+
+    def fork(self, slot, n):
+        """n fresh slots that hold what `slot` holds (its tokens so far), and the copies that make it so: [(tensor, its companion or None,
+        [from], [to])], blocks numbered along the second dimension of each tensor.  The copies are to be queued before anything else touches
+        the slots.  Nothing changes if the slots or the pages do not suffice."""
+        if not self.slots.is_held(slot):
+            raise CacheError("slot %r is not held by a live sequence" % (slot,))
+        if n < 0:
+            raise CacheError("%r sequences cannot go on from slot %r" % (n, slot))
+        if self.slots.n_free < n:
+            raise CacheFull("%d sequences wanted, %d slots free of %d" % (n, self.slots.n_free, self.n_slots))
+        length = self.seq_len[slot]
+        for g in self.kv_groups:
+            if g.fork_needs(length, n) > g.pool.n_free:
+                raise CacheFull("the fork needs %d more cache pages, %d are free of %d (max_tokens too small)"
+                                % (g.fork_needs(length, n), g.pool.n_free, g.n_pages))
+        new = [self.slots.acquire() for _ in range(n)]
+        copies = []
+        for s in new:
+            self.seq_len[s] = length
+        if new and length > 0:
+            for g in self.kv_groups:
+                pairs = g.fork_pages(slot, length, new)
+                if pairs:
+                    copies.append((g.k_pages, g.v_pages, [a for a, _ in pairs], [b for _, b in pairs]))
+                if g.sinks:
+                    copies.append((g.sink_k, g.sink_v, [slot] * n, new))
+                g.flush()
+        for g in self.state_groups if new else ():
+            copies.append((g.data, None, [slot] * n, new))
+        return new, copies
+
+    def cut(self, slots, lengths):
+        """Shortens sequences to the given lengths; the pages behind them are given back."""
+        for s, n in zip(slots, lengths):
+            if not self.slots.is_held(s) or not 0 <= n <= self.seq_len[s]:
+                raise CacheError("slot %r of %d tokens cannot be cut to %r" % (s, self.seq_len[s], n))
+        for s, n in zip(slots, lengths):
+            for g in self.kv_groups:
+                g.cut(s, self.seq_len[s], n)
+            self.seq_len[s] = n
+        for g in self.kv_groups:
+            g.flush()
 
     def tokens_held(self):
         return sum(pages_for(self.seq_len[s]) * PAGE for s in self.slots.held)

@@ -17,6 +17,9 @@
     Additions: --tokens 1,2,3 (prompt as token ids; with --batch-file one prompt a line),
       --batch-file <path>, --seed <int>, --dtype bfloat16|float32, --max-tokens <int>,
       --random <config.json> in place of the folder, --weight-seed <int> (default 0)
+      completion, what is drawn from: --top-k <int> (0: every token), --top-p <float> (1: all of their weight), --min-p <float> (0: off),
+      --samples <int> answers to every prompt (default 1), --draft <int>: guess that many tokens a step from the text itself and
+      keep those that the model agrees with (default 0: one token a step; the tokens are the same, up to rounding)
 
 Every option takes a value, as in the reference."""
 import math
@@ -48,10 +51,10 @@ def parse_args(argv):
     positional = not argv[0].startswith("--random")
     a = {"checkpoint": argv[0] if positional else "", "random": "", "weight_seed": 0, "device": "hip", "mode": "completion", "prompt": "", "prompt_path": "",
          "context": 0, "num_steps": 256, "temperature": 1.0, "n_junk": 250, "passkey_pos": -1, "tokens": "",
-         "batch_file": "", "seed": None, "dtype": "bfloat16", "max_tokens": 0}
+         "batch_file": "", "seed": None, "dtype": "bfloat16", "max_tokens": 0, "top_k": 0, "top_p": 1.0, "min_p": 0.0, "samples": 1, "draft": 0}
     i = 1 if positional else 0
     long_opts = {"--random": "random", "--weight-seed": "weight_seed", "--tokens": "tokens", "--batch-file": "batch_file", "--seed": "seed", "--dtype": "dtype",
-                 "--max-tokens": "max_tokens"}
+                 "--max-tokens": "max_tokens", "--top-k": "top_k", "--top-p": "top_p", "--min-p": "min_p", "--samples": "samples", "--draft": "draft"}
     while i < len(argv):
         flag = argv[i]
         if i + 1 >= len(argv):
@@ -59,7 +62,7 @@ def parse_args(argv):
         val = argv[i + 1]
         if flag in long_opts:
             key = long_opts[flag]
-            a[key] = int(val) if key in ("seed", "max_tokens", "weight_seed") else val
+            a[key] = int(val) if key in ("seed", "max_tokens", "weight_seed", "top_k", "samples", "draft") else float(val) if key in ("top_p", "min_p") else val
         elif len(flag) != 2 or flag[0] != "-":
             error_usage("unknown option %s" % flag)
         elif flag[1] == "h":
@@ -87,6 +90,10 @@ def parse_args(argv):
         else:
             error_usage("unknown option %s" % flag)
         i += 2
+    if a["top_k"] < 0 or not 0 <= a["top_p"] <= 1 or not 0 <= a["min_p"] <= 1 or a["samples"] < 1 or a["draft"] < 0:
+        error_usage("--top-k and --draft are 0 or more, --top-p and --min-p between 0 and 1, --samples 1 or more")
+    if a["draft"] and a["samples"] > 1:
+        error_usage("--draft and --samples do not go together")
     if a["dtype"] not in ("bfloat16", "float32"):
         error_usage("--dtype must be bfloat16 or float32")
     if bool(a["random"]) == bool(a["checkpoint"]):
@@ -163,13 +170,16 @@ def _prompts(a, model):
 def _engine(a, model, need_tokens, positions=None):
     from .engine import Engine
     budget = a["max_tokens"] or need_tokens
-    return Engine(model, max_tokens=max(64, budget), positions=positions if a["context"] else None)
+    return Engine(model, max_tokens=max(64, budget), positions=positions if a["context"] else None, max_draft=a["draft"] + 1 if a["draft"] else 0)
 
 
 def run_completion(a):
     """src/main.cpp:54-148."""
+    from .drafting import generate_drafted
     from .generate import GenerationStats, generate
     model = _load(a)
+    if a["draft"] and not model.takes_drafts():
+        error_usage("--draft is not offered for this model (its layers carry state, keep attention sinks or add a term by the distance)")
     prompts, tok = _prompts(a, model)
     max_len = model.spec.max_positions
     steps = a["num_steps"]
@@ -178,15 +188,15 @@ def run_completion(a):
     if a["context"]:                                                # under -T a text may run past the model's positions
         max_len = max(max_len, max(len(p) for p in prompts) + steps)
     held = (a["context"] // 64 + 2) * 64 if a["context"] else max_len      # a window's ring of pages holds no more
-    need = sum(min(max_len, len(p) + steps, max(held, len(p))) + 64 for p in prompts)
+    need = sum(min(max_len, len(p) + steps + a["draft"], max(held, len(p))) + 64 for p in prompts) * a["samples"]
     engine = _engine(a, model, need, positions=max_len)
     seed = a["seed"] if a["seed"] is not None else int(time.time() * 1000)          # main.cpp:66
     stats = GenerationStats()
     stop = list(model.spec.eos_token_ids)
     if tok is not None and tok.eot_id >= 0:
         stop.append(tok.eot_id)
-    last = {i: p[-1] for i, p in enumerate(prompts)}
-    single = len(prompts) == 1
+    last = {a["samples"] * i + k: p[-1] for i, p in enumerate(prompts) for k in range(a["samples"])}
+    single = len(last) == 1
 
     def on_token(i, t):
         if single:
@@ -201,19 +211,23 @@ def run_completion(a):
         model.weight_bytes() + sum(g.bytes_per_token() * (g.window or engine.n_positions) for g in engine.cache.kv_groups)))
     # graphs for the decode steps to come are captured before the clock starts (main.cpp:81-85 warms up too)
     shortest, longest = min(len(p) for p in prompts), min(max_len, max(len(p) for p in prompts) + steps)
-    sizes = list(range(1, min(len(prompts), engine.cache.n_slots) + 1))
+    sizes = list(range(1, min(len(last), engine.cache.n_slots) + 1)) if not a["draft"] else []
     from .engine import StepError
     try:
         engine.warmup(sizes, min_len=shortest + 1, max_len=longest)
     except StepError:                                   # more bucket pairs than the engine keeps: the full batch only
         engine.warmup(sizes[-1:], min_len=shortest + 1, max_len=min(longest, 2 * shortest + 64))
     t0 = time.perf_counter()
-    out = generate(engine, prompts, max_new_tokens=steps, temperature=a["temperature"], seed=seed, stop_ids=stop,
-                   on_token=on_token, stats=stats)
+    how = dict(max_new_tokens=steps, temperature=a["temperature"], seed=seed, stop_ids=stop, on_token=on_token, stats=stats,
+               top_k=a["top_k"], top_p=a["top_p"], min_p=a["min_p"])
+    if a["draft"]:
+        out = generate_drafted(engine, prompts, max_nodes=a["draft"] + 1, **how)
+    else:
+        out = generate(engine, prompts, samples=a["samples"], **how)
     elapsed = time.perf_counter() - t0
     if not single:
         for i, o in enumerate(out):
-            text = b"".join(tok.decode_one(p, t) for p, t in zip([prompts[i][-1]] + o[:-1], o)).decode(
+            text = b"".join(tok.decode_one(p, t) for p, t in zip([prompts[i // a["samples"]][-1]] + o[:-1], o)).decode(
                 "utf-8", "replace") if tok is not None else " ".join(map(str, o))
             print("[%d] %s" % (i, text))
     total = stats.prompt_tokens + stats.new_tokens

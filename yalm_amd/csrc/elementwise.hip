@@ -235,7 +235,7 @@ __global__ __launch_bounds__(ROPE_JOBS * WAVE) void rope_kv_write_kernel(const f
                                      T* __restrict__ v_stage, const int* __restrict__ seq_tile0,
                                      T* __restrict__ k_pages, T* __restrict__ v_pages,
                                      const int* __restrict__ block_table, int table_stride, int ring_pages,
-                                     const int* __restrict__ tok_seq, const int* __restrict__ tok_pos,
+                                     const int* __restrict__ tok_seq, const int* __restrict__ tok_pos, const int* __restrict__ tok_line,
                                      const int* __restrict__ seq_slot, const int* __restrict__ seq_len,
                                      const float2* __restrict__ cos_sin, int n_positions, int n_heads,
                                      int n_kv_heads, int hd, int rotary_dim, int n_pages, int page_layout, int slices,
@@ -312,6 +312,7 @@ __global__ __launch_bounds__(ROPE_JOBS * WAVE) void rope_kv_write_kernel(const f
   T* vpage = nullptr;
   int g = (job - n_heads) % n_kv_heads;
   bool is_k = (job - n_heads) < n_kv_heads;
+  if (tok_line != nullptr) pos = tok_line[t];    // a drafted token's place in the cache is not its position
   int r = pos & (PAGE - 1);
   if (slot >= 0 && pos >= 0 && k_pages != nullptr) {
     int ap = pos / PAGE;
@@ -564,12 +565,12 @@ extern "C" int yalm_rope_kv_write_tiles(const float* qkv, void* q_out, void* k_s
   return launch_status();
 }
 
-extern "C" int yalm_rope_kv_write(const float* qkv, void* q_out, void* k_stage, void* v_stage,
-                                  const int* seq_tile0, void* k_pages, void* v_pages, const int* block_table, int table_stride, int ring_pages,
-                                  const int* tok_seq, const int* tok_pos, const int* seq_slot, const int* seq_len,
-                                  const float* cos_sin, int n_positions, int T, int n_heads, int n_kv_heads,
-                                  int head_dim, int rotary_dim, int n_pages, int page_layout, int slices, int dtype,
-                                  hipStream_t stream) {
+extern "C" int yalm_rope_kv_write_lines(const float* qkv, void* q_out, void* k_stage, void* v_stage,
+                                        const int* seq_tile0, void* k_pages, void* v_pages, const int* block_table, int table_stride,
+                                        int ring_pages, const int* tok_seq, const int* tok_pos, const int* tok_line, const int* seq_slot,
+                                        const int* seq_len, const float* cos_sin, int n_positions, int T, int n_heads, int n_kv_heads,
+                                        int head_dim, int rotary_dim, int n_pages, int page_layout, int slices, int dtype,
+                                        hipStream_t stream) {
   if (T <= 0) return YALM_OK;
   if (head_dim <= 0 || (head_dim & 1) || rotary_dim < 0 || (rotary_dim & 1) || rotary_dim > head_dim ||
       n_heads <= 0 || n_kv_heads <= 0 || ring_pages <= 0 || slices < 1 || !page_layout_ok(page_layout, head_dim))
@@ -579,14 +580,25 @@ extern "C" int yalm_rope_kv_write(const float* qkv, void* q_out, void* k_stage, 
   if (dtype == YALM_F32)
     rope_kv_write_kernel<float><<<grid, ROPE_JOBS * WAVE, 0, stream>>>(
         qkv, (float*)q_out, (float*)k_stage, (float*)v_stage, seq_tile0, (float*)k_pages, (float*)v_pages, block_table,
-        table_stride, ring_pages, tok_seq, tok_pos, seq_slot, seq_len, (const float2*)cos_sin, n_positions, n_heads,
+        table_stride, ring_pages, tok_seq, tok_pos, tok_line, seq_slot, seq_len, (const float2*)cos_sin, n_positions, n_heads,
         n_kv_heads, head_dim, rotary_dim, n_pages, page_layout, slices, plane);
   else if (dtype == YALM_BF16)
     rope_kv_write_kernel<bf16><<<grid, ROPE_JOBS * WAVE, 0, stream>>>(
         qkv, (bf16*)q_out, (bf16*)k_stage, (bf16*)v_stage, seq_tile0, (bf16*)k_pages, (bf16*)v_pages, block_table, table_stride,
-        ring_pages, tok_seq, tok_pos, seq_slot, seq_len, (const float2*)cos_sin, n_positions, n_heads, n_kv_heads,
+        ring_pages, tok_seq, tok_pos, tok_line, seq_slot, seq_len, (const float2*)cos_sin, n_positions, n_heads, n_kv_heads,
         head_dim, rotary_dim, n_pages, page_layout, slices, plane);
   else
     return YALM_ERR_DTYPE;
   return launch_status();
+}
+
+extern "C" int yalm_rope_kv_write(const float* qkv, void* q_out, void* k_stage, void* v_stage,
+                                  const int* seq_tile0, void* k_pages, void* v_pages, const int* block_table, int table_stride, int ring_pages,
+                                  const int* tok_seq, const int* tok_pos, const int* seq_slot, const int* seq_len,
+                                  const float* cos_sin, int n_positions, int T, int n_heads, int n_kv_heads,
+                                  int head_dim, int rotary_dim, int n_pages, int page_layout, int slices, int dtype,
+                                  hipStream_t stream) {
+  return yalm_rope_kv_write_lines(qkv, q_out, k_stage, v_stage, seq_tile0, k_pages, v_pages, block_table, table_stride, ring_pages, tok_seq,
+                                  tok_pos, nullptr, seq_slot, seq_len, cos_sin, n_positions, T, n_heads, n_kv_heads, head_dim, rotary_dim,
+                                  n_pages, page_layout, slices, dtype, stream);
 }

@@ -165,6 +165,14 @@ int yalm_rope_kv_write(const float* qkv, void* q_out, void* k_stage, void* v_sta
                        int n_positions, int T, int n_heads, int n_kv_heads, int head_dim, int rotary_dim,
                        int n_pages, int page_layout, int slices, int dtype, hipStream_t stream);
 
+// yalm_rope_kv_write of tokens whose place in the cache is not their position: drafted tokens lie one behind the other, and several may
+// stand at one position.  q and k are turned by tok_pos[t]'s angles, k and v stored at position tok_line[t] (null: tok_pos[t]).
+int yalm_rope_kv_write_lines(const float* qkv, void* q_out, void* k_stage, void* v_stage, const int* seq_tile0,
+                             void* k_pages, void* v_pages, const int* block_table, int table_stride, int ring_pages, const int* tok_seq,
+                             const int* tok_pos, const int* tok_line, const int* seq_slot, const int* seq_len, const float* cos_sin,
+                             int n_positions, int T, int n_heads, int n_kv_heads, int head_dim, int rotary_dim,
+                             int n_pages, int page_layout, int slices, int dtype, hipStream_t stream);
+
 // The same for a step of whole prompts (every sequence from position 0; cu_seqlens [B + 1] token offsets,
 // n_tiles = seq_tile0[B]): whole page-shaped tiles at a time.  Needs a staging area; refuses
 // (YALM_ERR_ARG) head sizes whose transposed tile does not fit 64 KB of LDS.  slices as above.

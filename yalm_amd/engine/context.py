@@ -62,6 +62,15 @@ class Workspace:
         return sum(b.numel() * b.element_size() for b in list(self._flat.values()) + self._retired)
 
 
+class Draft:
+    """What a step of drafted tokens has beside the tensors of every step.  lines (int32 [T]): where a node's key and value lie in the
+    cache; mask (int64 [T, words]): the nodes that a node sees, itself among them; max_nodes, max_len: host values, the most nodes of a
+    sequence and its greatest length with them."""
+
+    def __init__(self, lines, mask, max_nodes, max_len):
+        self.lines, self.mask, self.max_nodes, self.max_len = lines, mask, max_nodes, max_len
+
+
 class StepContext:
     """mode: 'prefill' (sequences that start at position 0, whole prompts, packed)
     or 'decode' (one token per sequence, no slot in two rows: Engine.step and step_from refuse a batch that names one twice.  The kernels
@@ -78,7 +87,10 @@ class StepContext:
     pages_bucket: decode only; an upper bound (a power of two) of the pages of the step's
     longest sequence; with `ragged` (decode only: the step's sequences differ much in length, so that work
     cut per sequence would be uneven) the only way launch shapes may depend on lengths.
-    step_max_len: decode only; int32 [1] on the device, the length of the step's longest sequence.
+    draft: a step of drafted tokens only (mode 'draft': sequences that go on by a tree of tokens each, packed as prompts are; cu_seqlens
+    bounds their rows, tok_pos holds a node's position, its depth behind the sequence's tokens); a Draft.  Such a step reads and
+    writes the cache and no per-sequence state; parts that do not know the mode run in it what they run for any rows.
+    step_max_len: decode and draft only; int32 [1] on the device, the length of the step's longest sequence.
     seq_order: ragged decode steps only; int32 [B] on the device, the rows in the order in which a kernel whose
     work grows with a row's length should take them (the longest first, the second half from the shortest up)."""
 
@@ -94,6 +106,7 @@ class StepContext:
         self.normed = {}                  # id(norm part) -> (xn, ss, eps): activations a producer emitted for it
         self.pages_bucket = 1 << 30       # decode: no sequence of the step has more pages than this
         self.ragged = False
+        self.draft = None
         self.step_max_len = None
         self.seq_order = None
         self.max_position = 0

@@ -21,7 +21,7 @@ import torch
 
 from ..cache.manager import PAGE, CacheError, CacheManager
 from ..ops import kernels, library
-from .context import StepContext, Workspace
+from .context import Draft, StepContext, Workspace
 
 DECODE_BUCKETS = (1, 2, 4, 8, 16, 32, 64, 96, 128, 192, 256, 512, 1024)
 
@@ -81,12 +81,13 @@ class Engine:
     """max_tokens: the most tokens live sequences hold at any time (each rounded up to a page);
     max_batch: the most sequences alive at once; use_graphs: replay decode steps from captured
     graphs; max_graphs: the most (batch bucket, pages bucket) graphs kept (the least recently
-    used one goes first); positions: how far a sequence may run (default: the model's
+    used one goes first); max_draft: for models with a window, the most drafted tokens that a sequence goes on by in one draft_step
+    (the window's ring of pages keeps room for them; without a window there are always kernels.MAX_TREE_NODES); positions: how far a sequence may run (default: the model's
     max_position_embeddings) - more than the model's own only if every attention keeps a window,
     whose scores depend on distances alone (the reference's -T lets a text run on without end,
     src/infer.cpp:484-488)."""
 
-    def __init__(self, model, max_tokens, max_batch=None, use_graphs=True, max_graphs=24, positions=None):
+    def __init__(self, model, max_tokens, max_batch=None, use_graphs=True, max_graphs=24, positions=None, max_draft=0):
         if model.device is None:
             raise StepError("the model has no weights yet")
         if model.device.type != "cuda":
@@ -96,7 +97,10 @@ class Engine:
         self.device = model.device
         self.dtype = model.compute_dtype
         self.cache = CacheManager(model.cache_requests(), max_tokens, model.spec.max_positions, self.dtype,
-                                  self.device, n_slots=max_batch)
+                                  self.device, n_slots=max_batch, max_draft=min(int(max_draft), kernels.MAX_TREE_NODES) if model.takes_drafts() else 0)
+        windowed = any(g.window > 0 for g in self.cache.kv_groups)
+        self.max_draft = min(int(max_draft), kernels.MAX_TREE_NODES) if windowed else kernels.MAX_TREE_NODES
+        self._drafted = {}                              # slot -> (tokens held before, the parents of its drafted tokens)
         n_positions = model.spec.max_positions if self.cache.unbounded else \
             min(model.spec.max_positions, self.cache.max_seq_len)
         if positions is not None and int(positions) > n_positions:
@@ -129,7 +133,25 @@ class Engine:
 
     def release(self, slots):
         """Gives back what finished sequences hold."""
-        self.cache.release(list(slots))
+        slots = list(slots)
+        self.cache.release(slots)
+        for s in slots:
+            self._drafted.pop(s, None)
+
+    def fork(self, slot, n):
+        """n fresh slots that go on from what `slot` holds now (the same prompt answered several times).  Full pages of keys and values
+        are shared; the page that a sequence will write on in, a window's ring, sinks and per-sequence state are copied, in a launch
+        for each kind of cache line."""
+        if slot in self._drafted:
+            raise StepError("slot %r holds drafted tokens: keep some of them before others go on from it" % (slot,))
+        try:
+            new, copies = self.cache.fork(slot, int(n))
+        except CacheError as e:
+            raise StepError(str(e)) from None
+        for a, b, src, dst in copies:
+            both = torch.tensor([src, dst], dtype=torch.int32).to(self.device)
+            kernels.copy_pages(a, b, both[0], both[1])
+        return new
 
     def length(self, slot):
         return self.cache.seq_len[slot]
@@ -250,6 +272,105 @@ class Engine:
         new_lens = self._extend(slots, [1] * B, max(starts))
         return self._decode(slots, None, None, starts, new_lens, source, rows)
 
+    # ------------------------------------------------------------------ drafted tokens
+    def draft_step(self, slots, tokens, parents=None):
+        """A step in which every sequence goes on by a tree of tokens at once: tokens[i] are the nodes of slots[i], the first of them the
+        tree's root (the token that a plain step would bring), and parents[i][j] < j the node behind which node j stands (parents[i][0] is
+        not read; None: each behind the one before).  Node j stands at the position of its depth and sees the sequence's tokens, its
+        ancestors and itself.  Returns the logits behind every node, float32 [number of nodes of all, vocab], valid until the next step.
+        The sequences then hold their drafted tokens; keep() says which of them stay, before any other step of theirs."""
+        B = len(slots)
+        starts = self._starts(slots)
+        if not self.model.takes_drafts():
+            raise StepError("this model's layers do not take drafted tokens (they carry state from token to token, keep attention sinks or add a "
+                            "term by the distance)")
+        if len(tokens) != B or (parents is not None and len(parents) != B):
+            raise StepError("slots, tokens and parents must have the same length")
+        n_tok = [len(t) for t in tokens]
+        if min(n_tok) < 1 or max(n_tok) > self.max_draft:
+            raise StepError("a sequence goes on by 1 to %d drafted tokens (%s asked for; for a model with a window the engine's max_draft says how many)"
+                            % (self.max_draft, n_tok))
+        if min(starts) < 1:
+            raise StepError("a sequence goes on only after its prompt (lengths so far %s)" % (starts,))
+        V = self.model.vocab_size
+        bad = [tok for t in tokens for tok in t if not 0 <= tok < V]
+        if bad:
+            raise StepError("token id %r is outside the vocabulary of %d" % (bad[0], V))
+        words = (max(n_tok) + 63) // 64
+        T = sum(n_tok)
+        if T * max(self._widest_row, V) >= self.MAX_ELEMENTS:
+            raise StepError("a step of %d drafted tokens is refused: its widest buffer (%d elements a token) would reach 2^31 elements"
+                            % (T, max(self._widest_row, V)))
+        trees, depths, masks = [], [], np.zeros((T, words), dtype=np.uint64)
+        row = 0
+        for i, n in enumerate(n_tok):
+            up = list(range(-1, n - 1)) if parents is None else [-1] + [int(p) for p in parents[i][1:]]
+            if len(up) != n or any(not 0 <= up[j] < j for j in range(1, n)):
+                raise StepError("the parent of a drafted token is one in front of it (parents %s of %d tokens)" % (up, n))
+            depth, sees = [0] * n, [0] * n
+            for j in range(n):
+                sees[j] = 1 << j
+                if j:
+                    depth[j] = depth[up[j]] + 1
+                    sees[j] |= sees[up[j]]
+                for w in range(words):
+                    masks[row + j, w] = (sees[j] >> (64 * w)) & 0xFFFFFFFFFFFFFFFF
+            row += n
+            trees.append(up)
+            depths.append(depth)
+        narrowest = min([g.window for g in self.cache.kv_groups if g.window] + [1 << 30])
+        if max(d for ds in depths for d in ds) >= narrowest:
+            raise StepError("a tree as deep as the window of %d positions is refused" % narrowest)
+        max_pos = max(s + max(d) for s, d in zip(starts, depths))
+        new_lens = self._extend(slots, n_tok, max_pos)
+        cu = np.zeros(B + 1, dtype=np.int32)
+        np.cumsum(n_tok, out=cu[1:])
+        host = np.concatenate([np.asarray([tok for t in tokens for tok in t]), np.repeat(np.arange(B), n_tok),
+                               np.concatenate([np.asarray(d) + s for d, s in zip(depths, starts)]), np.asarray(slots), np.asarray(new_lens), cu,
+                               np.concatenate([np.arange(n) + s for n, s in zip(n_tok, starts)]), [max(new_lens)]]).astype(np.int32)
+        meta = self.ws.get("meta", (len(host),), torch.int32)
+        meta.copy_(torch.from_numpy(host))
+        mask = self.ws.get("draft.mask", (T, words), torch.int64)
+        mask.copy_(torch.from_numpy(masks.view(np.int64)))
+        ctx = self._context("draft", self.ws, meta, T, B, max_pos)
+        o = 3 * T + 3 * B + 1
+        ctx.draft = Draft(meta[o:o + T], mask, max(n_tok), max(new_lens))
+        ctx.step_max_len = meta[o + T:o + T + 1]
+        ctx.host_slots, ctx.host_n_tokens, ctx.host_start = list(slots), list(n_tok), list(starts)
+        for s, start, up in zip(slots, starts, trees):
+            self._drafted[s] = (start, up)
+        logits = self.ws.get("logits", (T, V), torch.float32)
+        self.model.forward(ctx, None, logits)
+        return logits
+
+    def keep(self, slots, paths):
+        """Ends a draft_step of these sequences: paths[i] are the drafted tokens of slots[i] that it goes on with, a path from the tree's root
+        downwards ([]: none of them).  Their keys and values move together behind the sequence's tokens, in one launch for each
+        kind of cache line, and the pages of the others are given back."""
+        if len(paths) != len(slots) or len(set(slots)) != len(slots):
+            raise StepError("keep needs one path for each of its slots, and each slot once")
+        starts = []
+        for s, path in zip(slots, paths):
+            if s not in self._drafted:
+                raise StepError("slot %r holds no drafted tokens" % (s,))
+            start, up = self._drafted[s]
+            if any(not 0 <= j < len(up) for j in path) or (len(path) > 0 and path[0] != 0) or any(up[b] != a for a, b in zip(path, path[1:])):
+                raise StepError("%s is no path from the root of the drafted tokens (parents %s)" % (list(path), up))
+            starts.append(start)
+        moving = [i for i, path in enumerate(paths) if any(j != k for k, j in enumerate(path))]
+        if moving:
+            cu = np.zeros(len(moving) + 1, dtype=np.int32)
+            np.cumsum([len(paths[i]) for i in moving], out=cu[1:])
+            n = len(moving)
+            host = np.concatenate([[slots[i] for i in moving], [starts[i] for i in moving], cu] + [np.asarray(paths[i]) for i in moving]).astype(np.int32)
+            meta = torch.from_numpy(host).to(self.device)
+            for g in self.cache.kv_groups:
+                kernels.compact_lines(g.k_pages, g.v_pages, g.table, g.ring_pages, meta[:n], meta[n:2 * n], meta[2 * n:3 * n + 1], meta[3 * n + 1:],
+                                      max(len(paths[i]) for i in moving))
+        for s in slots:
+            del self._drafted[s]
+        self.cache.cut(slots, [start + len(path) for start, path in zip(starts, paths)])
+
     def _starts(self, slots):
         """The lengths so far of the sequences of a step, after the checks on its slots."""
         B = len(slots)
@@ -260,6 +381,10 @@ class Engine:
         if not self.cache.slots.holds_all(slots):
             bad = [s for s in slots if not self.cache.slots.is_held(s)]
             raise StepError("slot %r is not held by a live sequence" % (bad[0],))
+        if self._drafted:
+            bad = [s for s in slots if s in self._drafted]
+            if bad:
+                raise StepError("slot %r holds drafted tokens: say which of them stay (keep) before it goes on" % (bad[0],))
         seq_len = self.cache.seq_len
         return [seq_len[s] for s in slots]
 

@@ -184,6 +184,13 @@ class Model:
                 out.append((safe, u, u + 1))
         return out
 
+    def takes_drafts(self):
+        """Whether steps of drafted tokens can run: nothing but keys and values is kept of a sequence, and every block's mixer attends to
+        trees of tokens (a block says so with `takes_drafts`)."""
+        if getattr(self.embedding, "cache_request", lambda: None)() is not None:
+            return False
+        return all(getattr(self.blocks[e.layer], "takes_drafts", False) for e in self.schedule)
+
     def describe(self):
         """({line on the kernels that serve a part: the schedule entries it stands for}, the lines that
         name a slow fallback), at the model's compute dtype."""

@@ -70,9 +70,11 @@ def plan_batches(prompt_lens, max_new_tokens, batch_size, max_tokens, n_slots, m
 
 
 def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_ids=None, batch_size=None,
-             sampler=None, on_token=None, stats=None, request_ids=None, ahead=None):
+             sampler=None, on_token=None, stats=None, request_ids=None, ahead=None, top_k=0, top_p=1.0, min_p=0.0, samples=1):
     """Generates for every prompt (a list of token ids).  Returns the new tokens of
-    each request, in the order of the prompts.  stop_ids None means the model's own
+    each request, in the order of the prompts.  top_k, top_p, min_p: see Sampler.draw.  samples > 1: every prompt is answered that many
+    times and runs once (its sequence is forked behind the prompt step); the answers of prompt i are the requests samples * i, samples * i + 1,
+    ... of the result and of on_token, drawn as requests of the ids samples * id, samples * id + 1, ...  stop_ids None means the model's own
     (config eos); on_token(request index, token) is called for every new token.
     ahead: queue each step before the host has read the tokens of the step before
     (default: if the engine has step_from and the sampler has draw).  A request that has ended
@@ -97,6 +99,13 @@ def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_
         ahead = can_ahead
     elif ahead and not can_ahead:
         raise ValueError("running a step ahead needs an engine with step_from and a sampler with draw")
+    samples = int(samples)
+    if samples < 1:
+        raise ValueError("every prompt is answered once at least (samples %d)" % samples)
+    if samples > 1:
+        prompts = [p for p in prompts for _ in range(samples)]
+        ids = [samples * r + k for r in ids for k in range(samples)]
+    filters = {} if (top_k, top_p, min_p) == (0, 1.0, 0.0) else {"top_k": top_k, "top_p": top_p, "min_p": min_p}
     results = [[] for _ in prompts]
     if max_new_tokens <= 0 or not prompts:
         return results
@@ -105,22 +114,34 @@ def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_
     for batch in plan:
         stats.batches += 1
         stats.batch_sizes.append(len(batch))
-        slots = engine.start(len(batch))
-        live = list(zip(batch, slots))
+        # the answers to one prompt that are in this batch: the first of them brings the prompt
+        firsts = [k for k, i in enumerate(batch) if k == 0 or i // samples != batch[k - 1] // samples]
+        slots = engine.start(len(firsts))
         held = set(slots)
         try:
             t0 = time.perf_counter()
-            logits = engine.step(slots, [prompts[i] for i in batch])
+            logits = engine.step(slots, [prompts[batch[k]] for k in firsts])
             stats.bytes_read += step_bytes(slots)
+            if len(firsts) < len(batch):
+                counts = [b - a for a, b in zip(firsts, firsts[1:] + [len(batch)])]
+                every = []
+                for s, n in zip(slots, counts):
+                    more = engine.fork(s, n - 1)
+                    held.update(more)
+                    every += [s] + more
+                import torch
+                logits = logits[torch.repeat_interleave(torch.arange(len(slots)), torch.tensor(counts)).to(logits.device)]
+                slots = every
+            live = list(zip(batch, slots))
             landed = None
             if ahead:
-                drawn = sampler.draw(logits, temperature, [ids[i] for i, _ in live], [0] * len(live))
+                drawn = sampler.draw(logits, temperature, [ids[i] for i, _ in live], [0] * len(live), **filters)
                 tokens = None
                 landed = drawn.tolist()                   # waits for the prompt step: its clock stops on the device's time
             else:
-                tokens = sampler.sample(logits, temperature, [ids[i] for i, _ in live], [0] * len(live))
+                tokens = sampler.sample(logits, temperature, [ids[i] for i, _ in live], [0] * len(live), **filters)
             stats.prefill_seconds += time.perf_counter() - t0
-            stats.prompt_tokens += sum(len(prompts[i]) for i in batch)
+            stats.prompt_tokens += sum(len(prompts[batch[k]]) for k in firsts)
             stats.batches_first_tokens += len(batch)
             t0 = time.perf_counter()
             rows = list(range(len(live)))                 # where each live sequence's token lies in the last draw
@@ -144,7 +165,7 @@ def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_
                     draw_ids = [ids[i] for i, _ in going]
                     draw_steps = [len(results[i]) + 1 for i, _ in going]
                     if ahead:
-                        next_drawn = sampler.draw(logits, temperature, draw_ids, draw_steps)
+                        next_drawn = sampler.draw(logits, temperature, draw_ids, draw_steps, **filters)
                 if ahead:                                 # lands while the step just queued runs (a batch's first
                     tokens = drawn.tolist() if landed is None else landed       # draw was read with the prompt step)
                     landed = None
@@ -169,7 +190,7 @@ def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_
                     engine.release(ended)
                     held.difference_update(ended)
                 if going and not ahead:                   # sampled only now: the tokens just appended are not in it
-                    next_tokens = sampler.sample(logits, temperature, draw_ids, draw_steps)
+                    next_tokens = sampler.sample(logits, temperature, draw_ids, draw_steps, **filters)
                 live, rows, drawn, tokens = still, still_rows, next_drawn, next_tokens
         except BaseException:
             engine.release(sorted(held))                  # a failed batch gives back what it still holds

@@ -540,10 +540,11 @@ def _check_heads(n_heads, n_kv_heads, head_dim):
 
 
 def rope_kv_write(qkv, q_out, k_stage, v_stage, seq_tile0, k_pages, v_pages, block_table, ring_pages, tok_seq, tok_pos,
-                  seq_slot, seq_len, cos_sin, n_heads, n_kv_heads, head_dim, rotary_dim, slices=1, layout=None):
+                  seq_slot, seq_len, cos_sin, n_heads, n_kv_heads, head_dim, rotary_dim, slices=1, layout=None, tok_line=None):
     """Rotates q and k by the angles of `cos_sin` at each token's position, writes q in
     q_out's dtype, k and v into the staging area (page format, tile seq_tile0[sequence] +
-    position // PAGE) if one is given, and into the pages of the cache if given.
+    position // PAGE) if one is given, and into the pages of the cache if given.  tok_line (int32 [T], without a staging
+    area): the places in the cache of tokens that do not lie at their positions (drafted ones).
     slices > 1: qkv is the flat scratch of gemm_partial, [slices][T][q + 2 kv] float32, and the
     slices are added while they are read."""
     _check_heads(n_heads, n_kv_heads, head_dim)
@@ -589,6 +590,14 @@ def rope_kv_write(qkv, q_out, k_stage, v_stage, seq_tile0, k_pages, v_pages, blo
         p_cs = _need(cos_sin, "cos_sin", torch.float32, (n_pos, rotary_dim // 2, 2))
     else:
         rotary_dim = 0
+    if tok_line is not None:
+        if k_stage is not None:
+            raise ValueError("rope_kv_write: a staging area holds whole prompts, whose tokens lie at their positions")
+        library.check(library.lib().yalm_rope_kv_write_lines(
+            p_qkv, p_q, p_ks, p_vs, p_t0, p_kp, p_vp, p_bt, stride, max(ring_pages, 1), p_ts, p_tp, _need(tok_line, "tok_line", torch.int32, (T,)),
+            p_ss, p_sl, p_cs, n_pos, T, n_heads, n_kv_heads, head_dim, rotary_dim, n_pages, _layout(layout, head_dim), int(slices),
+            dtype_code(dt), _stream()), "rope_kv_write")
+        return
     library.check(library.lib().yalm_rope_kv_write(
         p_qkv, p_q, p_ks, p_vs, p_t0, p_kp, p_vp, p_bt, stride, max(ring_pages, 1), p_ts, p_tp, p_ss, p_sl, p_cs,
         n_pos, T, n_heads, n_kv_heads, head_dim, rotary_dim, n_pages, _layout(layout, head_dim), int(slices),

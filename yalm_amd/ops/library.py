@@ -37,6 +37,7 @@ _SIGNATURES = {
     "yalm_gemm_f32_split_choice": (_I, [_I, _I, _I, _I]),
     "yalm_gemm_chain_qkv_rope": (_I, [_P, _P, _I, _F, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "yalm_rope_kv_write": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "yalm_rope_kv_write_lines": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "yalm_gemm_partial": (_I, [_P, _P, _P, ctypes.c_long, _I, _I, _I, _P, _P]),
     "yalm_gemm_bf16_dma_workspace": (ctypes.c_long, [_I, _I, _I]),
     "yalm_gemm_bf16_dma_choice": (_I, [_I, _I, _I, ctypes.c_long, _I]),
@@ -123,7 +124,7 @@ _SIGNATURES = {
     "yalm_probe_mfma": (_I, [_I, _I, _I, _P, _P, _P]),
 }
 
-ABI_VERSION = 47
+ABI_VERSION = 48
 
 
 class KernelError(RuntimeError):

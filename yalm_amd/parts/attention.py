@@ -224,6 +224,12 @@ class GQAttention(Part):
         return decode_splits(self.n_heads, self.n_kv_heads, self.head_dim, B, max_pages, ragged, shaped=hasattr(self.position, "score_bias"),
                              own=self.wo is not None and self.wo.dtype == torch.float32)
 
+    @property
+    def takes_drafts(self):
+        """Whether a step of drafted tokens (StepContext: mode 'draft') can run here: not beside sinks, which are stored as a sequence
+        passes them, nor with a term by the distance, which attn_tree does not add."""
+        return not self.sinks and not hasattr(self.position, "score_bias")
+
     def fuses_norm(self, norm, x, ctx):
         if not hasattr(norm, "fused") or self.head_dim % 16:
             return False
@@ -315,6 +321,14 @@ class GQAttention(Part):
         else:
             self._gemm(ctx, o, self.wo, x, kernels.EPI_ADD_F32)
 
+    def _draft_attention(self, q, o, ctx, group, k_pages, v_pages):
+        """Trees of drafted tokens over the cache, which holds their keys and values too."""
+        d, heads = ctx.draft, (self.n_heads, self.n_kv_heads, self.head_dim)
+        n_splits = kernels.attn_tree_splits(ctx.seq_slot.shape[0], d.max_nodes, d.max_len, *heads, q.dtype, self.window)
+        partial = ctx.ws.get("attn.partial", (kernels.attn_tree_workspace_floats(q.shape[0], self.n_heads, self.head_dim, n_splits),), torch.float32)
+        kernels.attn_tree(q, k_pages, v_pages, group.table, group.ring_pages, ctx.seq_slot, ctx.seq_len, ctx.cu_seqlens, d.mask, o, partial, *heads,
+                          self.window, n_splits, d.max_nodes, positions=ctx.tok_pos, step_max_len=ctx.step_max_len)
+
     def _decode_attention(self, q, o, ctx, group, line, k_pages, v_pages, writes_cache):
         T = q.shape[0]
         n_splits = self.decode_splits(T, min(group.ring_pages, ctx.pages_bucket), ctx.ragged)
@@ -344,7 +358,7 @@ class GQAttention(Part):
         prefill = ctx.mode == "prefill"
         n_qkv = self.q_dim + 2 * self.kv_dim
         slices = 1
-        if prefill and kernels.can_gemm_partial(T, self.dim, act):
+        if (prefill or ctx.draft is not None) and kernels.can_gemm_partial(T, self.dim, act):
             # the product's K slices (a short prompt's has some) go to the rotation kernel as they are, which adds them
             qkv = ws.get("gemm.partial", (kernels.fused_workspace_floats(T, n_qkv, self.dim),), torch.float32)
             slices = kernels.gemm_partial(h, self.wqkv, qkv)
@@ -404,7 +418,8 @@ class GQAttention(Part):
             if not done:
                 kernels.rope_kv_write(qkv, q, kst, vst, seq_tile0, k_pages, v_pages, group.table,
                                       group.ring_pages, ctx.tok_seq, ctx.tok_pos, ctx.seq_slot, ctx.seq_len, pos.table,
-                                      self.n_heads, self.n_kv_heads, self.head_dim, pos.rotary_dim, slices=slices)
+                                      self.n_heads, self.n_kv_heads, self.head_dim, pos.rotary_dim, slices=slices,
+                                      tok_line=None if ctx.draft is None else ctx.draft.lines)
         else:
             kernels.rope_kv_write(qkv, q, None, None, None, None, None, None, 0, ctx.tok_seq, ctx.tok_pos,
                                   ctx.seq_slot, ctx.seq_len, pos.table, self.n_heads, self.n_kv_heads, self.head_dim,
@@ -423,5 +438,7 @@ class GQAttention(Part):
                 sink_k, sink_v = group.line_sinks(line)
                 kernels.attn_sink_mix(q, o, lse, sink_k, sink_v, ctx.tok_seq, ctx.tok_pos, ctx.seq_slot, pos.table,
                                       self.n_heads, pos.rotary_dim, self.window, src_f32=o32)
+        elif ctx.draft is not None:
+            self._draft_attention(q, o, ctx, group, k_pages, v_pages)
         else:
             self._decode_attention(q, o, ctx, group, line, k_pages, v_pages, writes_cache)

@@ -31,6 +31,11 @@ class PreNormResidualBlock(Part):
         return [c for c in (self.mixer_norm, self.mixer_input, self.mixer, self.feed_forward_norm, self.feed_forward)
                 if c is not None]
 
+    @property
+    def takes_drafts(self):
+        """Whether the layer runs in a step of drafted tokens: its mixer does, and no filter in front of it carries state."""
+        return self.mixer_input is None and getattr(self.mixer, "takes_drafts", False)
+
     def cache_request(self):
         """What the layer keeps for a sequence: the mixer's, and beside it what the filter in front of the mixer keeps."""
         if self.mixer_input is None:

@@ -5,6 +5,8 @@ float32 logits on the device.  Randomness is explicit: the uniform number of a
 draw is a function of (seed, request id, step) alone, so a request's tokens do
 not depend on what else is in its batch (the reference seeds the C library's
 global generator with the wall clock, src/main.cpp:66, src/sampler.cpp:6-9)."""
+import math
+
 import torch
 
 from ..ops import kernels
@@ -52,32 +54,65 @@ class Sampler:
 
     def __init__(self, seed=0):
         self.seed = int(seed)
+        self._scratch = None      # workspace of the draws under filters
         self._host = []           # pinned buffers and the events after the copies into them, used in turn
         self._turn = 0
 
     def _host_buffers(self, R):
         """The next pinned pair in turn: int32 for the tokens on their way back, float32 for the
-        uniform numbers on their way out, and the event behind the draw that used them last."""
+        uniform numbers and the rows' settings on their way out, and the event behind the draw that used them last."""
         if len(self._host) < self.HOST_BUFFERS:
             n = max(R, 64)
             self._host.append([torch.empty(n, dtype=torch.int32, pin_memory=True),
-                               torch.empty(n, dtype=torch.float32, pin_memory=True), torch.cuda.Event()])
+                               torch.empty(5 * n, dtype=torch.float32, pin_memory=True), torch.cuda.Event()])
             return self._host[-1]
         entry = self._host[self._turn % self.HOST_BUFFERS]
         entry[2].synchronize()
         if entry[0].shape[0] < R:
             entry[0] = torch.empty(R, dtype=torch.int32, pin_memory=True)
-            entry[1] = torch.empty(R, dtype=torch.float32, pin_memory=True)
+            entry[1] = torch.empty(5 * R, dtype=torch.float32, pin_memory=True)
         return entry
 
-    def draw(self, logits, temperature, request_ids, steps):
-        """One token for each row of logits [R, vocab] (device, float32); temperature 0 is argmax.
+    def _filtered(self, logits, out, host, settings, request_ids, steps):
+        """sample_filtered with the rows' numbers and settings uploaded together, and a workspace kept from draw to draw (draws of one
+        sampler follow each other on one stream)."""
+        R, V = logits.shape
+        rows = host[:5 * R].view(5, R)
+        rows[0] = torch.tensor([uniform(self.seed, r, s) for r, s in zip(request_ids, steps)], dtype=torch.float32)
+        for i, (name, value) in enumerate(settings.items()):
+            whole = name == "top_k"
+            if isinstance(value, (int, float)):
+                value = [value] * R
+            value = [int(v) if whole else float(v) for v in value]
+            if len(value) != R:
+                raise ValueError("%s: %d settings for %d rows" % (name, len(value), R))
+            low, high = {"temperature": (0.0, math.inf), "top_k": (0, 2 ** 31 - 1), "top_p": (0.0, 1.0), "min_p": (0.0, 1.0)}[name]
+            if not all(low <= v <= high for v in value):
+                raise ValueError("%s: %s is not between %s and %s" % (name, value, low, high))
+            at = rows[1 + i]
+            (at.view(torch.int32) if whole else at).copy_(torch.tensor(value, dtype=torch.int32 if whole else torch.float32))
+        dev = torch.empty((5, R), dtype=torch.float32, device=logits.device)
+        dev.copy_(rows, non_blocking=True)                # from pinned memory: the host does not wait for the queue
+        need = kernels.sample_filtered_workspace(R, V)
+        if self._scratch is None or self._scratch.numel() < need or self._scratch.device != logits.device:
+            self._scratch = torch.empty(max(need, 1), dtype=torch.int32, device=logits.device)
+        kernels.sample_filtered(logits, dev[0], out, temperature=dev[1], top_k=dev[2].view(torch.int32), top_p=dev[3], min_p=dev[4],
+                                workspace=self._scratch)
+
+    def draw(self, logits, temperature, request_ids, steps, top_k=0, top_p=1.0, min_p=0.0):
+        """One token for each row of logits [R, vocab] (device, float32); temperature 0 is argmax.  top_k (0: off), top_p (1: off) and
+        min_p (0: off) leave a part of the tokens to draw from (kernels.sample_filtered); they and the temperature are numbers for all rows
+        or sequences of one for each.
         Nothing waits for the device here: the tokens can feed the next step from where they lie
         while the host reads them a step later."""
         R = logits.shape[0]
+        settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+        filtered = settings != {"temperature": temperature, "top_k": 0, "top_p": 1.0, "min_p": 0.0} or not isinstance(temperature, (int, float))
         out = torch.empty(R, dtype=torch.int32, device=logits.device)
         host, host_u, landed = self._host_buffers(R)
-        if temperature == 0.0:
+        if filtered:
+            self._filtered(logits, out, host_u, settings, request_ids, steps)
+        elif temperature == 0.0:
             kernels.argmax(logits, out)
         else:
             host_u[:R] = torch.tensor([uniform(self.seed, r, s) for r, s in zip(request_ids, steps)],
@@ -90,9 +125,9 @@ class Sampler:
         self._turn += 1
         return Drawn(out, host[:R], landed, self, self._turn)
 
-    def sample(self, logits, temperature, request_ids, steps):
+    def sample(self, logits, temperature, request_ids, steps, **filters):
         """As draw, but returns the tokens as a list of ints."""
-        return self.draw(logits, temperature, request_ids, steps).tolist()
+        return self.draw(logits, temperature, request_ids, steps, **filters).tolist()
 
     def argmax(self, logits):
         out = torch.empty(logits.shape[0], dtype=torch.int32, device=logits.device)
