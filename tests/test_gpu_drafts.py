@@ -197,7 +197,7 @@ def test_copied_pages_pass_over_what_is_no_page_and_copy_none():
     a = torch.arange(24.0, device=DEV).view(2, 4, 3)
     want = a.clone()
     want[:, 2] = a[:, 1]
-    K().copy_pages(a, None, i32([1, 0, 9, -1, 0]), i32([2, 7, 3, 3, -5]))
+    K().copy_pages(a, None, i32([1, 0, 9, -1, 0, 4]), i32([2, 7, 3, 3, -5, 2]))
     assert torch.equal(a, want)
     K().copy_pages(a, None, i32([]), i32([]))
     assert torch.equal(a, want)
