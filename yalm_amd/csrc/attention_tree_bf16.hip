@@ -3,14 +3,24 @@
 
 namespace {
 
+// The columns that a workgroup takes.
+int tree_columns(int B, int max_nodes, int n_heads, int n_kv_heads, int head_dim) {
+  const long cols = (long)max_nodes * (n_heads / n_kv_heads);
+  if (cols <= 16) return 16;
+  if (cols <= 32 || head_dim % 32 != 0) return 32;
+  if (cols <= 64) return 64;
+  return cols > 128 && 2l * B * n_kv_heads >= compute_units() ? 256 : 128;
+}
+
 // ---------------------------------------------------------------------------
-// More columns: a workgroup of two groups of four waves takes 64 NC columns, a wave 16 NC of them; the groups take every second
-// page of a split, which goes from memory straight into LDS (pages in blocks lie there as they are read: a fragment is 1 KB of
-// consecutive bytes), the next one in flight while this one is multiplied; the second group hands its results to the first at
-// the end.
+// More columns: eight waves share a run of pages, which go from memory straight into LDS two at a time (pages in blocks lie there as
+// they are read: a fragment is 1 KB of consecutive bytes), the next two in flight while these are multiplied.  With up to 64 NC columns
+// two groups of four waves take a page each and the second hands its results to the first at the end; with more (`wide`, up
+// to 128 NC) all eight waves split the columns and take both pages.  A wave has the tiles wave, wave + 4 (wide: + 8), ... of 16
+// columns, and leaves out those that the sequence does not fill.
 // ---------------------------------------------------------------------------
 template <int HD, int NC>
-__global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int chunks) {
+__global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int chunks, int wide_chunks) {
   typedef TreeColumns<bf16, HD, NC> C;
   static_assert(HD % 32 == 0, "pages in blocks");
   constexpr int DT = C::DT, TILE = PAGE * HD;      // elements of a page of a head
@@ -19,16 +29,30 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
   const TreeWork w(a, chunks);
   if (!w.any) return;
   const TreeSeq s(a, w.b);
-  const int G = a.n_heads / a.n_kv_heads, cols = min(s.nodes, a.max_nodes) * G, x0 = w.chunk * NC * 64;
+  const int G = a.n_heads / a.n_kv_heads, x0 = w.chunk * (wide_chunks ? NC * 128 : NC * 64);
+  const int cols = min(min(s.nodes, a.max_nodes) * G, x0 + (wide_chunks ? NC * 128 : NC * 64));
   if (x0 >= cols) return;
+  const bool wide = cols - x0 > NC * 64;
   const int half = __builtin_amdgcn_readfirstlane(threadIdx.x / 256), tid = threadIdx.x % 256;
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE, qd = lane / 16, j = lane % 16;
+  // the wave's first tile, and from tile to tile (columns)
+  const int mine = x0 + (wide ? wave + 4 * half : wave) * 16, step = wide ? 128 : 64;
+  const int tiles = __builtin_amdgcn_readfirstlane(min(NC, max(0, (cols - mine + step - 1) / step)));
   C col;
-  col.begin(a, s, w.g, x0 + wave * 16 * NC, cols, lane);
-  __shared__ int least[4];
-  if (half == 0 && lane == 0) least[wave] = col.lo_least;
+  col.begin(a, s, w.g, mine, step, cols, lane);
+  __shared__ int least[8], most[8];
+  if (lane == 0) {
+    least[wave + 4 * half] = col.lo_least;
+    most[wave + 4 * half] = col.lo_most;
+  }
   __syncthreads();
-  const int lo = min(min(least[0], least[1]), min(least[2], least[3]));
+  int lo = least[0], lo_most = most[0];
+#pragma unroll
+  for (int v = 1; v < 8; ++v) {
+    lo = min(lo, least[v]);
+    lo_most = max(lo_most, most[v]);
+  }
+  lo_most = col.lo_most = __builtin_amdgcn_readfirstlane(lo_most);       // which pages are at an edge is the workgroup's matter
   const TreePages pages(a, s, w.split, __builtin_amdgcn_readfirstlane(min(lo, s.base)) / PAGE);
   const float scale = 1.4426950408889634f / sqrtf((float)HD);
   const size_t page_elems = (size_t)a.n_kv_heads * PAGE * HD;
@@ -38,34 +62,86 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
 #if defined(__HIP_DEVICE_COMPILE__)
     const size_t at = (size_t)__builtin_amdgcn_readfirstlane(tree_page(a, s, page)) * page_elems;
     unsigned char* to = smem_raw + (size_t)((buf * 2 + half) * 2) * TILE * sizeof(bf16);
+    const int here = from_here(tid);
 #pragma unroll
     for (int p = 0; p < NLOAD; ++p) {
-      __builtin_amdgcn_global_load_lds(k0 + at + (tid + p * 256) * 8, to + (wave + p * 4) * 1024, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(v0 + at + (tid + p * 256) * 8, to + TILE * sizeof(bf16) + (wave + p * 4) * 1024, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(k0 + at + (here + p * 256) * 8, to + (wave + p * 4) * 1024, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(v0 + at + (here + p * 256) * 8, to + TILE * sizeof(bf16) + (wave + p * 4) * 1024, 16, 0, 0);
     }
 #endif
   };
-  const bool live = x0 + wave * 16 * NC < cols;    // a wave without columns only fetches
   if (pages.begin + half < pages.end) fetch(pages.begin + half, 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  int buf = 0;
-  for (int first = pages.begin; first < pages.end; first += 2, buf ^= 1) {
-    const int ap = first + half;
-    if (ap + 2 < pages.end) fetch(ap + 2, buf ^ 1);          // read before the last barrier
-    if (ap < pages.end && live) {
-      const bf16* ks = reinterpret_cast<const bf16*>(smem_raw) + (size_t)((buf * 2 + half) * 2) * TILE;
-      const bf16* vs = ks + TILE;
-      auto values = [&](int dt, int t) { return ld8(vs + C::value_place(dt, t, qd, j)); };
-      col.page(a, s, ap, qd, scale, [&](int t, int k) { return ld8(ks + C::key_place(t, k, qd, j)); }, values, values, []() {});
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // this wave's share of the next page has landed
-    __syncthreads();
-  }
+  // The walk over the pages two by two, for waves with N tiles: each number its own loops, with the registers that they need, and the
+  // rounds between the first and the last ones whose pages every column sees whole in a loop of their own.
+  const int rounds = (pages.end - pages.begin + 1) / 2;
+  const int whole = min(rounds, max(0, ((lo_most + PAGE - 1) / PAGE - pages.begin + 1) / 2));
+  const int behind = pages.end <= s.base / PAGE ? rounds : min(rounds, max(whole, (s.base / PAGE - pages.begin) / 2));
+  bool odd = false;
+  auto walk = [&](auto tiles_tag) {
+    constexpr int N = decltype(tiles_tag)::value;
+    auto go = [&](int from, int to, auto edge_tag) {
+      constexpr bool EDGE = decltype(edge_tag)::value;
+      for (int round = from; round < to; ++round) {
+        const int first = pages.begin + 2 * round, buf = round & 1;
+        if (first + half + 2 < pages.end) fetch(first + half + 2, buf ^ 1);      // read before the last barrier
+        // Values at an edge of what is seen: those behind the sequence, and those that are no finite numbers, are 0 from here on (0 times
+        // what they are is not always 0); the latter are read again behind the walk, for the columns that see them.
+        if constexpr (EDGE) {
+          bool mine_odd = false;
+          const int here = from_here(tid);
+          if (first + half < pages.end) {
+            bf16* vs = reinterpret_cast<bf16*>(smem_raw) + (size_t)((buf * 2 + half) * 2 + 1) * TILE;
+            const int left = s.len - (first + half) * PAGE;
+#pragma unroll
+            for (int p = 0; p < NLOAD; ++p) {
+              const int piece = here + p * 256, key = piece % 4 * 8 + piece / (4 * HD) * 32;         // eight keys of an element
+              bf16x8 v = ld8(vs + piece * 8);
+              bool changed = false;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const bool none = key + e >= left, finite = fabsf((float)v[e]) <= FLT_MAX;
+                mine_odd = mine_odd || (!finite && !none);
+                changed = changed || none || !finite;
+                if (none || !finite) v[e] = static_cast<bf16>(0.f);
+              }
+              if (changed) *reinterpret_cast<bf16x8*>(vs + piece * 8) = v;
+            }
+          }
+          odd = __syncthreads_or(mine_odd) || odd;
+        }
+        if constexpr (N > 0) {
+#pragma unroll 1
+          for (int which = wide ? 0 : half; which <= (wide ? 1 : half) && first + which < pages.end; ++which) {
+            const bf16* ks = reinterpret_cast<const bf16*>(smem_raw) + (size_t)((buf * 2 + which) * 2) * TILE;
+            const bf16* vs = ks + TILE;
+            col.template page<N, EDGE ? C::PART : C::WHOLE>(a, s, first + which, qd, scale,
+                                                            [&](int t, int k) { return ld8(ks + C::key_place(t, k, qd, j)); },
+                                                            [&](int dt, int t) { return ld8(vs + C::value_place(dt, t, qd, j)); }, []() {});
+          }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's share of the next pages has landed
+        __syncthreads();
+      }
+    };
+    go(0, whole, std::true_type{});
+    go(whole, behind, std::false_type{});
+    go(behind, rounds, std::true_type{});
+  };
+  if (tiles == NC) walk(std::integral_constant<int, NC>{});
+  else if (NC > 1 && tiles == 1) walk(std::integral_constant<int, 1>{});
+  else walk(std::integral_constant<int, 0>{});
+  if (odd)
+    for (int ap = pages.begin + (wide ? 0 : half); ap < pages.end; ap += wide ? 1 : 2)
+      if (col.at_edge(s, ap)) {
+        const bf16* vp = v0 + tree_page(a, s, ap) * page_elems;
+        col.add_odd(a, s, ap, qd, [&](int dt, int t) { return ld8(vp + C::value_place(dt, t, qd, j)); });
+      }
   // the second group hands its maxima, sums and results to the first, which merges and writes
   f32x4* mo = reinterpret_cast<f32x4*>(smem_raw);            // [NC][DT][256]
   float* ml = reinterpret_cast<float*>(mo + NC * DT * 256);  // [NC][2][256]
-  if (half == 1) {
+  if (!wide && half == 1) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
 #pragma unroll
@@ -75,20 +151,20 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
     }
   }
   __syncthreads();
-  if (half == 1) return;
+  if (!wide && half == 1) return;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const float m2 = ml[(c * 2) * 256 + tid], l2 = ml[(c * 2 + 1) * 256 + tid];
+    const float m2 = wide ? -FLT_MAX : ml[(c * 2) * 256 + tid], l2 = wide ? 0.f : ml[(c * 2 + 1) * 256 + tid];
     const float m = fmaxf(col.m[c], m2);
     const float f1 = __builtin_amdgcn_exp2f(col.m[c] - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
     const float lt = fold_column(col.l[c] * f1 + l2 * f2, [](float u, float v) { return u + v; });
-    const int x = x0 + (wave * NC + c) * 16 + j;
+    const int x = mine + c * step + j;
     if (x >= cols) continue;
     const size_t head = (size_t)(s.row0 + x / G) * a.n_heads + w.g * G + x % G;
     const float inv = tree_inverse(lt);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
-      tree_store<bf16, HD>(a, head, w.split, dt * 16 + 4 * qd, col.o[c][dt] * f1 + mo[(c * DT + dt) * 256 + tid] * f2, inv);
+      tree_store<bf16, HD>(a, head, w.split, dt * 16 + 4 * qd, wide ? col.o[c][dt] : col.o[c][dt] * f1 + mo[(c * DT + dt) * 256 + tid] * f2, inv);
     if (a.n_splits > 1 && qd == 0)
       *reinterpret_cast<float2*>(a.partial + (head * a.n_splits + w.split) * (HD + 2) + HD) = make_float2(m, lt);
   }
@@ -103,19 +179,20 @@ int launch_lds(const TreeArgs& a, hipStream_t stream) {
     static LdsAllowance allowed;
     if (int rc = allow_dynamic_lds(allowed, (const void*)kernel, lds); rc != YALM_OK) return rc;
   }
-  const int chunks = ((long)a.max_nodes * (a.n_heads / a.n_kv_heads) + NC * 64 - 1) / (NC * 64);
+  const int columns = tree_columns(a.B, a.max_nodes, a.n_heads, a.n_kv_heads, HD);
+  const int chunks = ((long)a.max_nodes * (a.n_heads / a.n_kv_heads) + columns - 1) / columns;
   const long units = (long)a.n_splits * a.n_kv_heads * a.B, groups = (units + 7) / 8 * 8 * chunks;
   if (groups > 0x7FFFFFFFl) return YALM_ERR_ARG;
-  kernel<<<(unsigned)groups, 512, lds, stream>>>(a, chunks);
+  kernel<<<(unsigned)groups, 512, lds, stream>>>(a, chunks, columns > NC * 64);
   return launch_status();
 }
 template <int HD>
 int launch_hd(const TreeArgs& a, hipStream_t stream) {
-  const long cols = (long)a.max_nodes * (a.n_heads / a.n_kv_heads);
-  if (cols <= 16) return launch_tree<bf16, HD, 1>(a, stream);
+  const int columns = tree_columns(a.B, a.max_nodes, a.n_heads, a.n_kv_heads, HD);
+  if (columns == 16) return launch_tree<bf16, HD, 1>(a, stream);
   if constexpr (HD % 32 == 0) {
-    if (cols > 64) return launch_lds<HD, 2>(a, stream);
-    if (cols > 32) return launch_lds<HD, 1>(a, stream);
+    if (columns > 64) return launch_lds<HD, 2>(a, stream);
+    if (columns > 32) return launch_lds<HD, 1>(a, stream);
   }
   return launch_tree<bf16, HD, 2>(a, stream);
 }

@@ -14,6 +14,13 @@
 
 namespace {
 
+// A lane's number as nothing can be known of it before here: what is worked out from it for a rare branch is worked out there, and
+// takes no registers from the loop around it.
+__device__ __forceinline__ int from_here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // the four lanes that share a column fold a value
 template <class F>
 __device__ __forceinline__ float fold_column(float v, F f) {
@@ -79,14 +86,14 @@ struct TreeColumns {
   float m[NC], l[NC];
   f32x4 o[NC][DT];
 
-  // columns x0 ... x0 + 16 NC - 1 of `cols`
-  __device__ __forceinline__ void begin(const TreeArgs& a, const TreeSeq& s, int g, int x0, int cols, int lane) {
+  // tiles of 16 columns from x0, x0 + step, ... of `cols`
+  __device__ __forceinline__ void begin(const TreeArgs& a, const TreeSeq& s, int g, int x0, int step, int cols, int lane) {
     const int qd = lane / 16, j = lane % 16, G = a.n_heads / a.n_kv_heads;
     lo_least = 0x7FFFFFFF;
     lo_most = 0;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int x = x0 + c * 16 + j;
+      const int x = x0 + c * step + j;
       const bool live = x < cols;
       row[c] = s.row0 + (live ? x / G : 0);
       const T* qr = (const T*)a.q + ((size_t)row[c] * a.n_heads + g * G + (live ? x % G : 0)) * HD;
@@ -123,34 +130,38 @@ struct TreeColumns {
     return BLOCKS ? (half * HD + dt * 16 + j) * 32 + value_key(t, qd) - 32 * half : (dt * 16 + j) * PAGE + value_key(t, qd);
   }
 
-  // A page.  keys(t, k) and values(dt, t) give a lane its fragments, again(dt, t) the values from where they come from (to hold
-  // them until then would cost registers), between() stands behind the last use of the keys.
-  template <class KF, class VF, class AF, class B>
-  __device__ __forceinline__ void page(const TreeArgs& a, const TreeSeq& s, int at, int qd, float scale, KF keys, VF values, AF again, B between) {
-    f32x4 sc[NC][4];
+  __device__ __forceinline__ bool at_edge(const TreeSeq& s, int at) const { return at * PAGE + PAGE > s.base || at * PAGE < lo_most; }
+
+  // A page, for the first N tiles of columns.  keys(t, k) and values(dt, t) give a lane its fragments, between() stands behind the
+  // last use of the keys.  EDGE: the page may be one at an edge of what the columns see (WHOLE: it is none; ANY: that is looked up here; PART:
+  // it may be one, and its values come without what must not reach the sums).  True: values of an edge page are no finite numbers (of
+  // a lane's); the sums went without them.
+  enum Edge { WHOLE, ANY, PART };
+  template <int N, Edge EDGE, class KF, class VF, class B>
+  __device__ __forceinline__ bool page(const TreeArgs& a, const TreeSeq& s, int at, int qd, float scale, KF keys, VF values, B between) {
+    f32x4 sc[N][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int c = 0; c < NC; ++c) sc[c][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < N; ++c) sc[c][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const Frag f = keys(t, k);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) sc[c][t] = X::mma(f, q[c][k], sc[c][t]);
+        for (int c = 0; c < N; ++c) sc[c][t] = X::mma(f, q[c][k], sc[c][t]);
       }
-    }
     between();
     const int p0 = at * PAGE;
-    const bool edge = p0 + PAGE > s.base || p0 < lo_most;
     // The probabilities as the second product's operands: in bfloat16 rounded, as the values are (a weighted mean moves by 2^-8
     // of a value at most, what its own rounding may move it by).
-    Frag pr[NC][KEYS];
-    float corr[NC];
-    unsigned seen[NC][2];                          // an edge page's keys that the column sees: the lane's eight of each half
-    bool settled = true;
+    Frag pr[N][KEYS];
+    float corr[N];
+    unsigned seen[N][2];                          // an edge page's keys that the column sees: the lane's eight of each half
     auto softmax = [&](auto masked) {
 #pragma unroll
-      for (int c = 0; c < NC; ++c) {
+      for (int c = 0; c < N; ++c) {
         float mx = -FLT_MAX;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -163,7 +174,6 @@ struct TreeColumns {
         mx = fold_column(mx, [](float u, float v) { return fmaxf(u, v); });
         const float m_new = fmaxf(m[c], mx * scale);
         corr[c] = __builtin_amdgcn_exp2f(m[c] - m_new);
-        settled = settled && corr[c] == 1.0f;
         float sum = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -177,67 +187,83 @@ struct TreeColumns {
         l[c] = l[c] * corr[c] + sum;
         m[c] = m_new;
       }
-      if constexpr (KEYS == 2) {
-        if (!__all(settled)) {                     // the maxima settle after a few pages
+      if constexpr (KEYS == 2) {                   // always: results in two places, one for a branch that leaves them, would cost their registers
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < N; ++c)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[c][dt] *= corr[c];
-        }
+          for (int dt = 0; dt < DT; ++dt) o[c][dt] *= corr[c];
       }
     };
     auto mix = [&](auto careful, auto tidy) {
+      if constexpr (KEYS == 2) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        if constexpr (decltype(careful)::value) __builtin_amdgcn_sched_barrier(0);       // a fragment at a time: registers are few
-        f32x4 part[NC];
-        if constexpr (KEYS != 2) {
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int c = 0; c < NC; ++c) part[c] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        }
+          for (int t = 0; t < KEYS; ++t) {
+            if constexpr (decltype(careful)::value) __builtin_amdgcn_sched_barrier(0);       // a fragment at a time: registers are few
+            const Frag f = tidy(values(dt, t), t);
 #pragma unroll
-        for (int t = 0; t < KEYS; ++t) {
-          const Frag f = tidy(values(dt, t), t);
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            if constexpr (KEYS == 2) o[c][dt] = X::mma(f, pr[c][t], o[c][dt]);
-            else part[c] = X::mma(f, pr[c][t], part[c]);
+            for (int c = 0; c < N; ++c) o[c][dt] = X::mma(f, pr[c][t], o[c][dt]);
           }
-        }
-        if constexpr (KEYS != 2) {
+      } else {
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
+        for (int dt = 0; dt < DT; ++dt) {
+          if constexpr (decltype(careful)::value) __builtin_amdgcn_sched_barrier(0);
+          f32x4 part[N];
+#pragma unroll
+          for (int c = 0; c < N; ++c) part[c] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < KEYS; ++t) {
+            const Frag f = tidy(values(dt, t), t);
+#pragma unroll
+            for (int c = 0; c < N; ++c) part[c] = X::mma(f, pr[c][t], part[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < N; ++c)
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[c][dt][r] = fmaf(o[c][dt][r], corr[c], part[c][r]);
         }
       }
     };
-    if (!edge) {
+    if (EDGE == WHOLE || (EDGE == ANY && !at_edge(s, at))) {
       softmax(std::false_type{});
       mix(std::false_type{}, [](Frag f, int) { return f; });
-      return;
+      return false;
     }
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const unsigned long long all = tree_seen(a, s, row[c], lo[c], at) >> (8 * qd);
+    for (int c = 0; c < N; ++c) {
+      const unsigned long long all = tree_seen(a, s, from_here(row[c]), lo[c], at) >> (8 * qd);
       seen[c][0] = (unsigned)all & 0xFF;
       seen[c][1] = (unsigned)(all >> 32) & 0xFF;
     }
     softmax(std::true_type{});
-    // Places behind the sequence may hold anything, and 0 times that is not always 0; nor is 0 times what is no finite number.  The
-    // products go without either, and where values are not finite the columns that see them get what they hold from products of
-    // ones that count them.
+    __builtin_amdgcn_sched_barrier(0);
+    // Places behind the sequence may hold anything, and 0 times that is not always 0; nor is 0 times what is no finite number.
     bool odd = false;
-    mix(std::true_type{}, [&](Frag f, int t) {
+    if constexpr (EDGE == PART) {
+      mix(std::false_type{}, [](Frag f, int) { return f; });
+    } else {
+      mix(std::true_type{}, [&](Frag f, int t) {
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        const bool none = p0 + value_key(t, qd) + e >= s.len, finite = fabsf(to_f32((T)f[e])) <= FLT_MAX;
-        odd = odd || (!finite && !none);
-        if (none || !finite) f[e] = from_f32<T>(0.f);
-      }
-      return f;
-    });
-    if (!__any(odd)) return;
+        for (int e = 0; e < PER; ++e) {
+          const bool none = p0 + value_key(t, qd) + e >= s.len, finite = fabsf(to_f32((T)f[e])) <= FLT_MAX;
+          odd = odd || (!finite && !none);
+          if (none || !finite) f[e] = from_f32<T>(0.f);
+        }
+        return f;
+      });
+    }
+    return odd;
+  }
+
+  // Values of an edge page that are no finite numbers, for the columns that see them: products of ones count them.  Behind all pages,
+  // which went without them: what they add is the same in any order, and the loop over the pages keeps its registers.
+  template <class AF>
+  __device__ __forceinline__ void add_odd(const TreeArgs& a, const TreeSeq& s, int at, int qd, AF again) {
+    const int p0 = at * PAGE;
+    unsigned long long all[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) all[c] = tree_seen(a, s, row[c], lo[c], at);
 #pragma unroll 1
     for (int kind = 0; kind < 3; ++kind) {         // no number, infinity, minus infinity
       const float what = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
@@ -261,13 +287,11 @@ struct TreeColumns {
           for (int t = 0; t < KEYS; ++t) {
             Frag sees;
 #pragma unroll
-            for (int e = 0; e < PER; ++e)
-              sees[e] = from_f32<T>((float)((KEYS == 2 ? seen[c][t] >> e : seen[c][t >> 1] >> (4 * (t & 1) + e)) & 1));
+            for (int e = 0; e < PER; ++e) sees[e] = from_f32<T>((float)((unsigned)(all[c] >> (value_key(t, qd) + e)) & 1));
             count = X::mma(ones[t], sees, count);
           }
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (count[r] > 0.f) o[c][dt][r] += what;
+          for (int r = 0; r < 4; ++r) o[c][dt][r] += count[r] > 0.f ? what : 0.f;
         }
       }
     }
@@ -331,7 +355,7 @@ __global__ __launch_bounds__(TREE_WAVES * WAVE, NC == 1 && sizeof(T) == 2 ? 2 : 
   if (x0 >= cols) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE, qd = lane / 16, j = lane % 16;
   C col;
-  col.begin(a, s, w.g, x0, cols, lane);
+  col.begin(a, s, w.g, x0, 16, cols, lane);
   const TreePages pages(a, s, w.split, __builtin_amdgcn_readfirstlane(min(col.lo_least, s.base)) / PAGE);
   const float scale = 1.4426950408889634f / sqrtf((float)HD);          // scores in exponents of 2
   const size_t page_elems = (size_t)a.n_kv_heads * PAGE * HD;
@@ -348,6 +372,7 @@ __global__ __launch_bounds__(TREE_WAVES * WAVE, NC == 1 && sizeof(T) == 2 ? 2 : 
   int ap = pages.begin + wave;
   int phys = ap < pages.end ? tree_page(a, s, ap) : 0;
   if (ap < pages.end) load_keys(phys);
+  bool odd = false;
   auto one_page = [&](auto has_next) {
     const T* vp = v0 + phys * page_elems;
     Frag vreg[DT][KEYS];
@@ -358,17 +383,24 @@ __global__ __launch_bounds__(TREE_WAVES * WAVE, NC == 1 && sizeof(T) == 2 ? 2 : 
     int physn = 0;
     if constexpr (decltype(has_next)::value) physn = tree_page(a, s, ap + NW);
     __builtin_amdgcn_sched_barrier(0);             // the values are asked for before the keys are waited for
-    col.page(a, s, ap, qd, scale, [&](int t, int k) { return kreg[t][k]; }, [&](int dt, int t) { return vreg[dt][t]; },
-             [&](int dt, int t) { return *reinterpret_cast<const Frag*>(vp + C::value_place(dt, t, qd, j)); }, [&]() {
+    const bool found = col.template page<NC, C::ANY>(a, s, ap, qd, scale, [&](int t, int k) { return kreg[t][k]; }, [&](int dt, int t) { return vreg[dt][t]; },
+                                                    [&]() {
       if constexpr (decltype(has_next)::value) {
         load_keys(physn);                          // they stay in flight while this page is mixed
         phys = physn;
         __builtin_amdgcn_sched_barrier(0);
       }
     });
+    odd = odd || __any(found);
   };
   for (; ap + NW < pages.end; ap += NW) one_page(std::true_type{});
   if (ap < pages.end) one_page(std::false_type{});
+  if (odd)
+    for (ap = pages.begin + wave; ap < pages.end; ap += NW)
+      if (col.at_edge(s, ap)) {
+        const T* vp = v0 + tree_page(a, s, ap) * page_elems;
+        col.add_odd(a, s, ap, qd, [&](int dt, int t) { return *reinterpret_cast<const Frag*>(vp + C::value_place(dt, t, qd, j)); });
+      }
 
   // the four lanes of a column hold parts of its sum; then the waves merge, a tile of columns at a time
   float factor[NC];

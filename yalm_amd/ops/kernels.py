@@ -902,7 +902,7 @@ def attn_tree_splits(n_seqs, max_nodes, max_len, n_heads, n_kv_heads, head_dim, 
     if dtype == torch.float32:
         tile, resident = (32 if cols > 16 and head_dim <= 96 else 16), 256
     elif cols > 32 and head_dim % 32 == 0:
-        tile, resident = (128 if cols > 64 else 64), 256
+        tile, resident = (64 if cols <= 64 else 256 if cols > 128 and 2 * n_seqs * n_kv_heads >= 256 else 128), 256
     else:
         tile, resident = (32, 256) if cols > 16 else (16, 512)
     pages = (max_len + PAGE - 1) // PAGE
