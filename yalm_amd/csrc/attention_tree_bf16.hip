@@ -13,8 +13,8 @@ int tree_columns(int B, int max_nodes, int n_heads, int n_kv_heads, int head_dim
 }
 
 // ---------------------------------------------------------------------------
-// More columns: eight waves share a run of pages, which go from memory straight into LDS two at a time (pages in blocks lie there as
-// they are read: a fragment is 1 KB of consecutive bytes), the next two in flight while these are multiplied.  With up to 64 NC columns
+// More columns: eight waves share a run of pages, which go from memory straight into LDS two at a time (pages in blocks: a fragment is 1 KB
+// of consecutive bytes), the next two in flight while these are multiplied.  With up to 64 NC columns
 // two groups of four waves take a page each and the second hands its results to the first at the end; with more (`wide`, up
 // to 128 NC) all eight waves split the columns and take both pages.  A wave has the tiles wave, wave + 4 (wide: + 8), ... of 16
 // columns, and leaves out those that the sequence does not fill.
@@ -62,11 +62,13 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
 #if defined(__HIP_DEVICE_COMPILE__)
     const size_t at = (size_t)__builtin_amdgcn_readfirstlane(tree_page(a, s, page)) * page_elems;
     unsigned char* to = smem_raw + (size_t)((buf * 2 + half) * 2) * TILE * sizeof(bf16);
-    const int here = from_here(tid);
+    // a fragment's 64 pieces of 16 bytes lie in the order of the lanes that read them (qd, j), not of their rows (j, qd): lanes that
+    // follow each other then read from all banks
+    const int here = from_here(lane), piece = wave * 64 + here % 16 * 4 + here / 16;
 #pragma unroll
     for (int p = 0; p < NLOAD; ++p) {
-      __builtin_amdgcn_global_load_lds(k0 + at + (here + p * 256) * 8, to + (wave + p * 4) * 1024, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(v0 + at + (here + p * 256) * 8, to + TILE * sizeof(bf16) + (wave + p * 4) * 1024, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(k0 + at + (piece + p * 256) * 8, to + (wave + p * 4) * 1024, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(v0 + at + (piece + p * 256) * 8, to + TILE * sizeof(bf16) + (wave + p * 4) * 1024, 16, 0, 0);
     }
 #endif
   };
@@ -96,7 +98,7 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
             const int left = s.len - (first + half) * PAGE;
 #pragma unroll
             for (int p = 0; p < NLOAD; ++p) {
-              const int piece = here + p * 256, key = piece % 4 * 8 + piece / (4 * HD) * 32;         // eight keys of an element
+              const int piece = here + p * 256, key = piece % 64 / 16 * 8 + piece / (4 * HD) * 32;      // eight keys of an element
               bf16x8 v = ld8(vs + piece * 8);
               bool changed = false;
 #pragma unroll
@@ -117,8 +119,8 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
             const bf16* ks = reinterpret_cast<const bf16*>(smem_raw) + (size_t)((buf * 2 + which) * 2) * TILE;
             const bf16* vs = ks + TILE;
             col.template page<N, EDGE ? C::PART : C::WHOLE>(a, s, first + which, qd, scale,
-                                                            [&](int t, int k) { return ld8(ks + C::key_place(t, k, qd, j)); },
-                                                            [&](int dt, int t) { return ld8(vs + C::value_place(dt, t, qd, j)); }, []() {});
+                                                            [&](int t, int k) { return ld8(ks + (k * 4 + t) * 512 + lane * 8); },
+                                                            [&](int dt, int t) { return ld8(vs + (t * DT + dt) * 512 + lane * 8); }, []() {});
           }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // this wave's share of the next pages has landed
