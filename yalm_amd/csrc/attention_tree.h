@@ -22,21 +22,31 @@ struct TreeArgs {
   const int* step_max_len;     // [1], or null
 };
 
+// A number of the step's tables, which no kernel writes while one reads them: where all lanes ask for the same one it comes by the
+// scalar cache, and no load of a page in flight is waited for with it.
+__device__ __forceinline__ int table_entry(const int* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return *(const __attribute__((address_space(4))) int*)p;
+#else
+  return *p;
+#endif
+}
+
 // A sequence of the step: its slot's row of the block table, its rows, its length (0 where it has no slot) and how many tokens it
 // held before the drafted ones.
 struct TreeSeq {
   int slot, row0, nodes, len, base;
   __device__ __forceinline__ TreeSeq(const TreeArgs& a, int b) {
-    slot = a.seq_slot[b];
-    row0 = a.cu_nodes[b];
-    nodes = min(a.cu_nodes[b + 1], a.T) - row0;
-    len = (unsigned)slot < (unsigned)a.n_slots ? a.seq_len[b] : 0;
+    slot = table_entry(a.seq_slot + b);
+    row0 = table_entry(a.cu_nodes + b);
+    nodes = min(table_entry(a.cu_nodes + b + 1), a.T) - row0;
+    len = (unsigned)slot < (unsigned)a.n_slots ? table_entry(a.seq_len + b) : 0;
     base = max(len - nodes, 0);
   }
 };
 
 __device__ __forceinline__ int tree_page(const TreeArgs& a, const TreeSeq& s, int page) {
-  return min(max(a.block_table[(size_t)s.slot * a.table_stride + page % a.ring_pages], 0), a.n_pages - 1);
+  return min(max(table_entry(a.block_table + (size_t)s.slot * a.table_stride + page % a.ring_pages), 0), a.n_pages - 1);
 }
 
 // The first of the sequence's own tokens that row r sees (base and more: none).  Without positions a row stands as many places behind

@@ -58,9 +58,9 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
   const size_t page_elems = (size_t)a.n_kv_heads * PAGE * HD;
   const bf16* k0 = (const bf16*)a.k_pages + (size_t)w.g * PAGE * HD;
   const bf16* v0 = (const bf16*)a.v_pages + (size_t)w.g * PAGE * HD;
-  auto fetch = [&](int page, int buf) {
+  auto fetch = [&](int phys, int buf) {          // phys: the page's place in the pool
 #if defined(__HIP_DEVICE_COMPILE__)
-    const size_t at = (size_t)__builtin_amdgcn_readfirstlane(tree_page(a, s, page)) * page_elems;
+    const size_t at = (size_t)__builtin_amdgcn_readfirstlane(phys) * page_elems;
     unsigned char* to = smem_raw + (size_t)((buf * 2 + half) * 2) * TILE * sizeof(bf16);
     // a fragment's 64 pieces of 16 bytes lie in the order of the lanes that read them (qd, j), not of their rows (j, qd): lanes that
     // follow each other then read from all banks
@@ -72,7 +72,10 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
     }
 #endif
   };
-  if (pages.begin + half < pages.end) fetch(pages.begin + half, 0);
+  // places are looked up a round ahead of the page's way into LDS: the one trip to memory would else wait for the other
+  auto place = [&](int page) { return page < pages.end ? tree_page(a, s, page) : 0; };
+  int ahead = place(pages.begin + half + 2);
+  if (pages.begin + half < pages.end) fetch(place(pages.begin + half), 0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   // The walk over the pages two by two, for waves with N tiles: each number its own loops, with the registers that they need, and the
@@ -87,7 +90,10 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
       constexpr bool EDGE = decltype(edge_tag)::value;
       for (int round = from; round < to; ++round) {
         const int first = pages.begin + 2 * round, buf = round & 1;
-        if (first + half + 2 < pages.end) fetch(first + half + 2, buf ^ 1);      // read before the last barrier
+        if (first + half + 2 < pages.end) {
+          fetch(ahead, buf ^ 1);                 // that buffer was read before the last barrier
+          ahead = place(first + half + 4);
+        }
         // Values at an edge of what is seen: those behind the sequence, and those that are no finite numbers, are 0 from here on (0 times
         // what they are is not always 0); the latter are read again behind the walk, for the columns that see them.
         if constexpr (EDGE) {

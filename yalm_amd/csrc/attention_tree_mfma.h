@@ -307,7 +307,7 @@ struct TreePages {
     const int last = (s.len - 1) / PAGE, total = last - first + 1;
     int per = (total + a.n_splits - 1) / a.n_splits;
     if (a.step_max_len != nullptr) {               // sequences of unequal lengths: pieces of the longest one's size, fewer of a short one
-      const int most = max(a.step_max_len[0], 1);
+      const int most = max(table_entry(a.step_max_len), 1);
       const int pages = (most - 1) / PAGE - (a.window > 0 ? max(0, most - a.max_nodes - a.window + 1) / PAGE : 0) + 1;
       per = max(per, (pages + a.n_splits - 1) / a.n_splits);
     }
