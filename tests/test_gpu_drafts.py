@@ -204,7 +204,7 @@ def test_copied_pages_pass_over_what_is_no_page_and_copy_none():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("hd,H,ring", [(128, 2, 4), (64, 1, 3), (48, 3, 3), (6, 1, 3), (96, 8, 5), (272, 1, 3)])
+@pytest.mark.parametrize("hd,H,ring", [(128, 2, 4), (64, 1, 3), (48, 3, 3), (6, 1, 3), (96, 8, 5), (272, 1, 3), (32, 2, 3), (160, 1, 3), (1024, 1, 3)])
 def test_kept_lines_move_together(hd, H, ring, dtype):
     """Paths of every length, the first and the last place of a page, a ring that wraps, a row without a slot; all else stays."""
     g = torch.Generator().manual_seed(hd)

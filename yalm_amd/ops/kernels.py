@@ -51,6 +51,8 @@ def _need(t, name, dtype=None, shape=None):
         if shape is None:
             return t.data_ptr()
         have = t.shape
+        if have == shape:                 # without a None in it the comparison in one piece: 0.35 us less of 1.06 an argument
+            return t.data_ptr()
         if len(have) == len(shape):
             for s, d in zip(shape, have):
                 if s is not None and s != d:
