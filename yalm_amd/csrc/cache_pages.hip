@@ -59,11 +59,11 @@ int launch_copy(void* a, void* b, int n_lines, int n_blocks, long block_bytes, c
 // ---------------------------------------------------------------------------
 // compaction: line start + keep[k] of a sequence to line start + k, k in turn, for keep ascending: place k is never the source
 // of a later move, so that a thread that owns one element of a head's keys and values moves them all without waiting for
-// anyone.  Grid (KV head, line, sequence).  What a move of 2-byte values costs is not their bytes: a value's elements lie 64 bytes apart
-// (pages in blocks) or more, so that a wave's load touches 64 pieces of memory for one element of each.  64 sequences that keep up to 7 of 40
-// tokens, 32 lines of 8 heads of 128 in bfloat16, move 198 MB where the tokens are 54, in 94 us (2.1 TB/s).  Half pages staged in LDS, read and
-// written 16 bytes at a time, took 93 us with a workgroup for a head (waiting at its barriers) and 155 with a wave for 64 elements (fewer
-// waves in flight), and were left.
+// anyone.  Grid (KV head, line, sequence).  What a move of 2-byte values costs is not their bytes but the memory
+// they lie in: a value's elements stand 64 bytes apart (pages in blocks) or more, so that every line of a half page is read and written for
+// one element of each.  64 sequences that keep up to 7 of 40 tokens, 32 lines of 8 heads of 128 in bfloat16, ask for 54 MB and take 95 us, with
+// some 240 MB read and 78 written.  Half pages staged in LDS, read and written 16 bytes at a time, took 93 us with a workgroup for a head and
+// 155 with a wave for 64 elements (fewer waves in flight), and were left.
 // ---------------------------------------------------------------------------
 constexpr int MOVES = 8;                         // moves a thread has in flight
 
