@@ -111,6 +111,29 @@ def test_filtered_sampling_of_odd_rows(V):
         check_sampled(logits, u, *draw_rows(logits, u, T, k, p, mp), T, k, p, mp, name)
 
 
+FAR = [(1.0, 769, 1.0, 0.0), (0.7, 1000, 0.95, 0.0), (1.0, 768, 0.9, 0.0), (0.6, 4000, 0.3, 0.05), (1.5, 9999, 0.9999, 0.0), (1.0, 800, 1e-9, 0.0),
+       (100.0, 2000, 0.5, 0.0), (1e-3, 2000, 0.5, 0.0), (3.0, 1500, 1.0, 0.3), (0.3, 60000, 0.99, 0.0), (1.0, 100000, 1.0, 0.0), (2.0, 20000, 0.75, 0.001)]
+
+
+@pytest.mark.parametrize("V", [770, 1000, 4097, 32001, 128256])
+@pytest.mark.parametrize("width", [0.5, 2.5, 12.0])
+def test_ranks_behind_many_tokens(V, width):
+    settings = FAR + [(0.9, V - 1, 0.97, 0.0), (0.9, V // 2, 1.0, 0.0)]
+    logits = rnd((len(settings), V), V + int(width), torch.float32, width)
+    u = np.random.default_rng(V).random(len(settings)).astype(np.float32)
+    T, k, p, mp = (list(x) for x in zip(*settings))
+    check_sampled(logits, u, *draw_rows(logits, u, T, k, p, mp), T, k, p, mp, "V %d" % V)
+
+
+@pytest.mark.parametrize("V", [1200, 20011])
+def test_ranks_behind_many_tokens_of_odd_rows(V):
+    for name, row in odd_rows(V, torch.Generator().manual_seed(V)).items():
+        logits = row.repeat(len(FAR), 1)
+        u = np.random.default_rng(V).random(len(FAR)).astype(np.float32)
+        T, k, p, mp = (list(x) for x in zip(*FAR))
+        check_sampled(logits, u, *draw_rows(logits, u, T, k, p, mp), T, k, p, mp, name)
+
+
 def test_rows_with_nothing_to_draw_and_settings_left_out():
     nothing = torch.stack([torch.full((50,), -float("inf")), torch.full((50,), float("nan"))]).to(DEV)
     out, prob = torch.zeros(2, dtype=torch.int32, device=DEV), torch.ones(2, device=DEV)

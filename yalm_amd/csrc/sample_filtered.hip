@@ -15,9 +15,9 @@
 // end is what makes them visible): the maxima of 1,024 interleaved groups of a row; then a row with a rank collects the tokens that
 // may have it (the k-th of the groups' maxima is no greater than the k-th of all tokens) and a row with a nucleus adds its weights
 // up by bins; then the kept weights of each chunk of the row, and the tokens of the border's bin; then one workgroup a row ranks
-// the collected tokens, finds the chunk in which the number falls and the token in it.  What this does not take - ranks beyond
-// MAX_RANK, more than LIST tokens to rank against each other - the last launch does as a call without a workspace does: one workgroup a
-// row over the whole row, whose borders are narrowed by the bits of the logits where many share a bin.
+// the collected tokens, finds the chunk in which the number falls and the token in it.  Ranks beyond MAX_RANK go the way of a nucleus: they
+// become a limit on the weight.  What this does not take - more than LIST tokens to rank against each other - the last launch does as a call
+// without a workspace does: one workgroup a row over the whole row, whose borders are narrowed by the bits of the logits where many share a bin.
 #include <float.h>
 #include <math.h>
 #include <type_traits>
@@ -35,6 +35,7 @@ constexpr int ROOTS = 32;
 constexpr int OCTAVES = 44;                      // the bins reach down to 2^-44 of the greatest weight
 constexpr int SEG = 192;                         // tokens of the list that a wave's run of the row may hold
 constexpr int BORDER = 768;                      // tokens of one bin that are ranked against each other
+constexpr int MAX_RANK = 768;                    // of 1,024 groups of a row: some 1,400 tokens reach the 768th of their maxima
 constexpr int GROUPS = BINS / NW;                // partial sums of the row that a wave leaves for the walk
 
 // A value moved between the lanes of a wave in its registers; lanes that nothing reaches get 0.
@@ -269,6 +270,7 @@ struct Wish {
   float T, p, mp, u;
   int k;
   bool by_rank, by_mass;
+  bool few, far;               // ranks whose tokens are collected, and ranks that lie behind more of them
   u64 least;                   // the weight of min_p
   __device__ __forceinline__ Wish(const Step& st, int row) {
     // asked for together: what is left out reads the row's number in its place
@@ -281,6 +283,8 @@ struct Wish {
     p = st.top_p != nullptr ? a : 1.f;
     mp = st.min_p != nullptr ? b : 0.f;
     by_rank = k > 0 && k < st.V;
+    few = by_rank && k <= MAX_RANK;
+    far = by_rank && k > MAX_RANK;
     by_mass = p < 1.f;
     const double f = mp > 0.f ? ceil(ldexp((double)fminf(mp, 1.f), st.scale)) : 0.0;
     least = f > 1.0 ? (u64)f : 1ull;
@@ -652,7 +656,6 @@ __global__ __launch_bounds__(NT) void sample_alone_kernel(Step st) {
 // ---------------------------------------------------------------------------
 constexpr int CHUNK = 4 * NT;                    // logits that a workgroup takes with one load a thread
 constexpr int MAX_GROUPS_ROW = 64;               // workgroups a row: a power of two
-constexpr int MAX_RANK = 768;                    // of 1,024 groups of a row: some 1,400 tokens reach the 768th of their maxima
 constexpr int LIST = 2048;                       // collected tokens that the last launch ranks
 constexpr int CHUNKS_EACH = 64;                  // chunks that a workgroup takes at most
 constexpr int MAX_CHUNKS = BINS;
@@ -664,6 +667,7 @@ struct Left {
   u64* mass;                   // [BINS]
   u64* list;                   // [LIST] ~key << 32 | index: rising numbers are the tokens' order
   u64* sums;                   // [chunks] kept weights
+  unsigned* counts;            // [BINS] tokens
   int* count;                  // collected tokens
   int* first;                  // the first of the greatest
   __device__ __forceinline__ Left(const Step& st, int row) {
@@ -671,13 +675,14 @@ struct Left {
     mass = reinterpret_cast<u64*>(at);
     list = mass + BINS;
     sums = list + LIST;
-    top = reinterpret_cast<float*>(sums + st.chunks);
+    counts = reinterpret_cast<unsigned*>(sums + st.chunks);
+    top = reinterpret_cast<float*>(counts + BINS);
     peak = top + NT;
     count = reinterpret_cast<int*>(peak + (size_t)st.chunks * NW);
     first = count + 1;
   }
 };
-inline long left_bytes(int chunks) { return ((BINS + LIST + chunks) * 8l + (NT + (long)chunks * NW) * 4l + 8 + 15) / 16 * 16; }
+inline long left_bytes(int chunks) { return ((BINS + LIST + chunks) * 8l + (BINS + NT + (long)chunks * NW) * 4l + 8 + 15) / 16 * 16; }
 
 // the thread's four logits of a chunk; behind the row's end no number
 __device__ __forceinline__ float4 chunk4(const Row& r, int chunk) {
@@ -743,7 +748,10 @@ __global__ __launch_bounds__(NT) void sample_top_kernel(Step st) {
   });
   for (int o = 1; o < n; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, WAVE));
   if (threadIdx.x % n == 0) left.top[blockIdx.x * (NT / n) + threadIdx.x / n] = mx;
-  for (int i = blockIdx.x * NT + threadIdx.x; i < BINS; i += n * NT) left.mass[i] = 0;
+  for (int i = blockIdx.x * NT + threadIdx.x; i < BINS; i += n * NT) {
+    left.mass[i] = 0;
+    left.counts[i] = 0;
+  }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     *left.count = 0;
     *left.first = 0x7FFFFFFF;
@@ -766,16 +774,18 @@ __device__ __forceinline__ float logit_of(u64 order) {
   return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
 }
 
-// Rows with a rank: the tokens up to the bin of the k-th of the groups' maxima.  Rows with a nucleus: weights by bins.
+// Rows with a rank: the tokens up to the bin of the k-th of the groups' maxima.  Rows with a nucleus or a far rank: weights by bins, and for
+// the rank the tokens by bins.
 __global__ __launch_bounds__(NT, 8) void sample_sift_kernel(Step st) {
   __shared__ double roots[ROOTS];
   __shared__ u64 mass[BINS];
+  __shared__ unsigned counts[BINS];
   __shared__ float red[NW];
   __shared__ unsigned waves[NW];
   __shared__ int border;
   const int row = blockIdx.y, tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
   const Wish want(st, row);
-  if (!(want.T > 0.f) || !(want.by_rank ? want.k <= MAX_RANK : want.by_mass)) return;
+  if (!(want.T > 0.f) || !(want.by_rank || want.by_mass)) return;
   fill_roots(roots);
   Row r = row_of(st, row, roots);
   const Left left(st, row);
@@ -783,15 +793,14 @@ __global__ __launch_bounds__(NT, 8) void sample_sift_kernel(Step st) {
   const float m = block_max<NW>(mine, red);
   if (!(m > -INFINITY)) return;
   set_scale(r, m, want.T);
-  if (want.by_rank) {
-    unsigned* count = reinterpret_cast<unsigned*>(mass);
-    count[tid] = count[tid + NT] = 0;
+  if (want.few) {
+    counts[tid] = counts[tid + NT] = 0;
     if (tid == 0) border = BINS - 1;
     __syncthreads();
     const int b = r.bin(mine);
-    if (b < BINS) atomicAdd(&count[b], 1u);
+    if (b < BINS) atomicAdd(&counts[b], 1u);
     __syncthreads();
-    const unsigned c0 = count[2 * tid], c1 = count[2 * tid + 1];
+    const unsigned c0 = counts[2 * tid], c1 = counts[2 * tid + 1];
     unsigned c = wave_scan(c0 + c1);
     if (lane == WAVE - 1) waves[wave] = c;
     __syncthreads();
@@ -813,21 +822,28 @@ __global__ __launch_bounds__(NT, 8) void sample_sift_kernel(Step st) {
     return;
   }
   mass[tid] = mass[tid + NT] = 0;
+  counts[tid] = counts[tid + NT] = 0;
   __syncthreads();
   chunks_of<4>(r, st.chunks, [&](int, float4 v) {
     const float l[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int b = r.bin(l[j]);
-      if (b < BINS) atomicAdd(&mass[b], r.weight(l[j]));
+      if (b < BINS) {
+        atomicAdd(&mass[b], r.weight(l[j]));
+        if (want.far) atomicAdd(&counts[b], 1u);
+      }
     }
   });
   __syncthreads();
-  for (int i = tid; i < BINS; i += NT)
+  for (int i = tid; i < BINS; i += NT) {
     if (mass[i] != 0) atomicAdd(&left.mass[i], mass[i]);
+    if (counts[i] != 0) atomicAdd(&left.counts[i], counts[i]);
+  }
 }
 
 // The bin in which the running mass reaches the limit, the mass in front of it, and the limit.
+constexpr int FOUND = 7;
 struct Border {
   int bin;
   u64 above, limit;
@@ -857,15 +873,78 @@ __device__ __forceinline__ Border find_border(const Left& left, const Wish& want
   return {(int)found[0], found[1], limit};
 }
 
-// Rows without a rank: the kept weights of each chunk (in front of the border's bin), and the tokens of that bin.
+// A far rank.  Its border's bin comes from the tokens by bins; the weight of the first k lies between that of the bins in front of it and that
+// of those with it, and so does what top_p leaves of it: the bins from `lo` to `hi` can hold the end of the prefix, and all in front is kept.
+// Without a nucleus that is the rank's bin.  A rank of 2,000 of 128,256: 29 us for a row, 33 for 8, 70 for 64 (one workgroup a row 101, 102 and
+// 113); of 20,000 with 0.9 of the weight 42, 49 and 90 (242, 246, 257).
+struct Far {
+  int rank, lo, hi;
+  int need;                    // tokens of the rank's bin that belong to the first k
+  u64 above_rank, above_lo;    // the mass in front
+};
+__device__ __forceinline__ Far far_borders(const Left& left, const Wish& want, u64* waves, u64* found) {
+  const int tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+  const uint2 n = reinterpret_cast<const uint2*>(left.counts)[tid];
+  const ulonglong2 a = reinterpret_cast<const ulonglong2*>(left.mass)[tid];
+  u64 c = wave_scan((u64)(n.x + n.y));
+  if (lane == WAVE - 1) waves[wave] = c;
+  if (tid == 0) {
+    found[0] = BINS;
+    found[1] = 0;
+  }
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) c += waves[w];
+  const u64 k = (u64)want.k, c1 = c - n.y, c0 = c1 - n.x;
+  if (c0 < k && c >= k) {
+    const bool second = c1 < k;
+    found[0] = 2 * tid + (second ? 1 : 0);
+    found[1] = k - (second ? c1 : c0);
+  }
+  __syncthreads();
+  Far f;
+  f.rank = (int)found[0];
+  f.need = (int)found[1];
+  u64 m = wave_scan((u64)(a.x + a.y));
+  if (lane == WAVE - 1) waves[wave] = m;
+  __syncthreads();
+  u64 total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < wave) m += waves[w];
+    total += waves[w];
+  }
+  const u64 m1 = m - a.y, m0 = m1 - a.x;
+  if (f.rank < BINS ? f.rank / 2 == tid : tid == 0) {
+    found[2] = f.rank == BINS ? total : (f.rank & 1) ? m1 : m0;
+    found[3] = f.rank == BINS ? total : (f.rank & 1) ? m : m1;
+  }
+  __syncthreads();
+  f.above_rank = f.above_lo = found[2];
+  f.lo = f.hi = f.rank;
+  if (!want.by_mass) return f;
+  const u64 least = want.mass_limit(f.above_rank), most = want.mass_limit(found[3]);
+  if (m0 < least && m >= least) {
+    found[4] = 2 * tid + (m1 < least ? 1 : 0);
+    found[5] = m1 < least ? m1 : m0;
+  }
+  if (m0 < most && m >= most) found[6] = 2 * tid + (m1 < most ? 1 : 0);
+  __syncthreads();
+  f.lo = (int)found[4];
+  f.above_lo = found[5];
+  f.hi = (int)found[6];
+  return f;
+}
+
+// Rows but for those with a collected rank: the kept weights of each chunk (in front of the border's bin), and the tokens of the bins in which
+// a border may lie.
 __global__ __launch_bounds__(NT, 8) void sample_sum_kernel(Step st) {
   __shared__ double roots[ROOTS];
   __shared__ float red[NW];
-  __shared__ u64 waves[NW], found[2];
+  __shared__ u64 waves[NW], found[FOUND];
   __shared__ u64 parts[CHUNKS_EACH][NW];
   const int row = blockIdx.y, tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
   const Wish want(st, row);
-  if (want.T > 0.f && want.by_rank) return;
+  if (want.T > 0.f && want.few) return;
   fill_roots(roots);
   Row r = row_of(st, row, roots);
   const Left left(st, row);
@@ -881,8 +960,16 @@ __global__ __launch_bounds__(NT, 8) void sample_sum_kernel(Step st) {
     return;
   }
   set_scale(r, m, want.T);
-  int bin = BINS;
-  if (want.by_mass) bin = find_border(left, want, waves, found).bin;
+  int bin = BINS, hi = BINS, rank = BINS;
+  if (want.far) {
+    const Far f = far_borders(left, want, waves, found);
+    bin = f.lo;
+    hi = f.hi;
+    rank = f.rank;
+  } else if (want.by_mass) {
+    bin = hi = rank = find_border(left, want, waves, found).bin;
+  }
+  auto border = [&](int b) { return b < BINS && ((b >= bin && b <= hi) || b == rank); };
   chunks_of<4>(r, st.chunks, [&](int chunk, float4 v) {
     const float l[4] = {v.x, v.y, v.z, v.w};
     int b[4];
@@ -895,9 +982,9 @@ __global__ __launch_bounds__(NT, 8) void sample_sum_kernel(Step st) {
         sum += w >= want.least ? w : 0;
       }
     }
-    if (bin < BINS && __any(b[0] == bin || b[1] == bin || b[2] == bin || b[3] == bin)) {
+    if (bin < BINS && __any(border(b[0]) || border(b[1]) || border(b[2]) || border(b[3]))) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) append(left, b[j] == bin, order_of(l[j], chunk * CHUNK + 4 * tid + j));
+      for (int j = 0; j < 4; ++j) append(left, border(b[j]), order_of(l[j], chunk * CHUNK + 4 * tid + j));
     }
     sum = wave_sum64(sum);
     if (lane == 0) parts[chunk / (int)gridDim.x][wave] = sum;
@@ -916,7 +1003,7 @@ struct Last {                                    // LDS of the last launch besid
   u64 a[LIST], b[LIST];
   u64 sums[MAX_CHUNKS];
   u64 fine[FINE];
-  u64 waves[NW], found[2], last;
+  u64 waves[NW], found[FOUND], last;
   float red[NW];
   int best, n;
 };
@@ -1025,11 +1112,11 @@ __global__ __launch_bounds__(NT) void sample_last_kernel(Step st) {
   const float top = left.top[tid];
   const u64 first = left.list[tid];
   __syncthreads();
-  if (!greedy && ((want.by_rank && want.k > MAX_RANK) || n > LIST)) {
+  if (!greedy && n > LIST) {
     row_alone(lds.alone, roots, st, row, want);
     return;
   }
-  if (!greedy && want.by_rank && n > 0 && n <= WAVE) {
+  if (!greedy && want.few && n > 0 && n <= WAVE) {
     if (wave == 0) last_of_few(st, row, want, r, s.a, first, n);
     return;
   }
@@ -1047,7 +1134,7 @@ __global__ __launch_bounds__(NT) void sample_last_kernel(Step st) {
   if (tid + NT < n) s.a[tid + NT] = left.list[tid + NT];
   auto weight = [&](u64 order) { return r.weight(logit_of(order)); };
   if (tid == 0) s.best = 0;
-  if (want.by_rank) {
+  if (want.few) {
     // all that can be drawn is in the list: the first k of it, the shortest prefix of those, down to min_p, in the order of indices
     __syncthreads();
     sort_rising(s.a, s.b, n);
@@ -1082,7 +1169,28 @@ __global__ __launch_bounds__(NT) void sample_last_kernel(Step st) {
     s.last = 0;
     s.n = 0;
   }
-  if (want.by_mass) {
+  if (want.far) {
+    // the collected tokens in their order: the rank's border gives the weight of the first k, that the limit, and the running sums the tokens
+    const Far f = far_borders(left, want, s.waves, s.found);
+    bin = f.lo;
+    __syncthreads();
+    sort_rising(s.a, s.b, n);
+    running_sums(s.b, n, s.waves, [&](int i) { return weight(s.a[i]); });
+    auto bin_at = [&](int i) { return r.bin(logit_of(s.a[i])); };
+    for (int i = tid; i < n; i += NT)
+      if (bin_at(i) == f.rank && (i == 0 || bin_at(i - 1) != f.rank)) s.n = i;
+    __syncthreads();
+    const int of_rank = s.n;
+    u64 limit = f.above_rank;
+    if (f.rank < BINS) limit += s.b[of_rank + f.need - 1] - (of_rank > 0 ? s.b[of_rank - 1] : 0);
+    if (want.by_mass) limit = want.mass_limit(limit);
+    for (int i = tid; i < n; i += NT)
+      if (bin_at(i) <= f.hi && f.above_lo + (i > 0 ? s.b[i - 1] : 0) < limit) {
+        const u64 w = weight(s.a[i]);
+        if (w >= want.least) atomicAdd(&s.sums[(unsigned)s.a[i] / CHUNK], w);
+        atomicMax(&s.last, s.a[i]);
+      }
+  } else if (want.by_mass) {
     for (int i = tid; i < FINE; i += NT) s.fine[i] = 0;
     const Border f = find_border(left, want, s.waves, s.found);
     bin = f.bin;
@@ -1152,7 +1260,7 @@ __global__ __launch_bounds__(NT) void sample_last_kernel(Step st) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int b = r.bin(l[j]);
-    const bool in = b < BINS && (b < bin || (b == bin && order_of(l[j], chunk * CHUNK + 4 * tid + j) <= border_last));
+    const bool in = b < BINS && (b < bin || order_of(l[j], chunk * CHUNK + 4 * tid + j) <= border_last);
     const u64 w = in ? r.weight(l[j]) : 0;
     a[j] = w >= want.least ? w : 0;
   }
