@@ -20,7 +20,14 @@ struct TreeArgs {
   float* partial;
   int T, B, n_heads, n_kv_heads, head_dim, window, n_splits, max_nodes, n_pages, page_layout;
   const int* step_max_len;     // [1], or null
+  unsigned group_inverse;      // 2^32 / (n_heads / n_kv_heads) and a part more: exact for the columns of groups up to MAX_GROUP
+  // the node of a sequence whose query a column is
+  __device__ __forceinline__ int node_of(int column) const {
+    return group_inverse == 0 ? column : (int)__umulhi((unsigned)column, group_inverse);
+  }
 };
+constexpr int MAX_NODES = 256;                     // of a sequence
+constexpr int MAX_GROUP = 4095;                    // column * (what the inverse is too great by) stays below 2^32
 
 // A number of the step's tables, which no kernel writes while one reads them: where all lanes ask for the same one it comes by the
 // scalar cache, and no load of a page in flight is waited for with it.

@@ -133,16 +133,17 @@ extern "C" int yalm_attn_tree(const void* q, const void* k_pages, const void* v_
                               int page_layout, int dtype, int force_simple, const int* step_max_len, hipStream_t stream) {
   if (T <= 0 || B <= 0) return YALM_OK;
   if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || head_dim <= 0 || head_dim > MAX_HD || ring_pages <= 0 ||
-      ring_pages > table_stride || n_slots <= 0 || n_pages <= 0 || mask_words <= 0 || n_splits <= 0 || max_nodes <= 0 || n_heads > 65535 ||
+      ring_pages > table_stride || n_slots <= 0 || n_pages <= 0 || mask_words <= 0 || n_splits <= 0 || max_nodes <= 0 || max_nodes > MAX_NODES || n_heads > 65535 ||
       !page_layout_ok(page_layout, head_dim))
     return YALM_ERR_ARG;
+  const int group = n_heads / n_kv_heads;
   const TreeArgs a = {q, k_pages, v_pages, block_table, table_stride, n_slots, ring_pages, seq_slot, seq_len, cu_nodes,
                       (const unsigned long long*)mask, mask_words, positions, out, partial, T, B, n_heads, n_kv_heads, head_dim, window,
-                      n_splits, max_nodes, n_pages, page_layout, step_max_len};
+                      n_splits, max_nodes, n_pages, page_layout, step_max_len, group == 1 ? 0u : (unsigned)((1ull << 32) / group + 1)};
   if (dtype != YALM_F32 && dtype != YALM_BF16) return YALM_ERR_DTYPE;
   // The matrix cores' kernels load and store 16 bytes a lane, from pages as the cache keeps them.
   const uintptr_t at = (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out | (n_splits > 1 ? (uintptr_t)partial : 0);
-  const bool cores = !force_simple && head_dim % 16 == 0 && head_dim <= 128 && (at & 15) == 0 &&
+  const bool cores = !force_simple && group <= MAX_GROUP && head_dim % 16 == 0 && head_dim <= 128 && (at & 15) == 0 &&
                      (page_layout == YALM_PAGE_BLOCKS) == (head_dim % 32 == 0);
   if (!cores) {
     if (dtype == YALM_F32) attn_tree_simple_kernel<float><<<dim3(T, n_heads), WAVE, 0, stream>>>(a);

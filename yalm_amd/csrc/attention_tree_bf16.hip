@@ -105,16 +105,8 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
 #pragma unroll
             for (int p = 0; p < NLOAD; ++p) {
               const int piece = here + p * 256, key = piece % 64 / 16 * 8 + piece / (4 * HD) * 32;      // eight keys of an element
-              bf16x8 v = ld8(vs + piece * 8);
-              bool changed = false;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const bool none = key + e >= left, finite = fabsf((float)v[e]) <= FLT_MAX;
-                mine_odd = mine_odd || (!finite && !none);
-                changed = changed || none || !finite;
-                if (none || !finite) v[e] = static_cast<bf16>(0.f);
-              }
-              if (changed) *reinterpret_cast<bf16x8*>(vs + piece * 8) = v;
+              words4 v = *reinterpret_cast<const words4*>(vs + piece * 8);
+              if (tidy_values(v, left - key, mine_odd)) *reinterpret_cast<words4*>(vs + piece * 8) = v;
             }
           }
           odd = __syncthreads_or(mine_odd) || odd;
@@ -168,7 +160,8 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
     const float lt = fold_column(col.l[c] * f1 + l2 * f2, [](float u, float v) { return u + v; });
     const int x = mine + c * step + j;
     if (x >= cols) continue;
-    const size_t head = (size_t)(s.row0 + x / G) * a.n_heads + w.g * G + x % G;
+    const int node = a.node_of(x);
+    const size_t head = (size_t)(s.row0 + node) * a.n_heads + w.g * G + x - node * G;
     const float inv = tree_inverse(lt);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)

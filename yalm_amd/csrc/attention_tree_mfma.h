@@ -71,6 +71,24 @@ struct TreeWork {
   }
 };
 
+// Eight values in bfloat16, of which the first `left` are the sequence's: the others and those that are no finite numbers become 0; `odd`
+// where there are some of the latter.  Words of two values each, on whole registers: an exponent of ones and one more at its end reach the
+// place of the sign.  True: something changed.
+typedef __attribute__((ext_vector_type(4))) unsigned words4;
+__device__ __forceinline__ bool tidy_values(words4& v, int left, bool& odd) {
+  unsigned ends[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) ends[e] = (v[e] & 0x7F807F80u) + 0x00800080u;
+  if (left >= 8 && ((ends[0] | ends[1] | ends[2] | ends[3]) & 0x80008000u) == 0) return false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const unsigned held = 2 * e + 1 < left ? ~0u : 2 * e < left ? 0xFFFFu : 0u, at = ends[e] & held & 0x80008000u;
+    odd = odd || at != 0;
+    v[e] &= held & ~((at << 1) - (at >> 15));      // from a half's sign place to all of the half
+  }
+  return true;
+}
+
 // The columns of a wave: queries, running maxima (exponents of 2), sums and results.
 template <typename T, int HD, int NC>
 struct TreeColumns {
@@ -95,8 +113,9 @@ struct TreeColumns {
     for (int c = 0; c < NC; ++c) {
       const int x = x0 + c * step + j;
       const bool live = x < cols;
-      row[c] = s.row0 + (live ? x / G : 0);
-      const T* qr = (const T*)a.q + ((size_t)row[c] * a.n_heads + g * G + (live ? x % G : 0)) * HD;
+      const int node = live ? a.node_of(x) : 0;
+      row[c] = s.row0 + node;
+      const T* qr = (const T*)a.q + ((size_t)row[c] * a.n_heads + g * G + (live ? x - node * G : 0)) * HD;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int e = k * STEP + qd * PER;
@@ -244,6 +263,11 @@ struct TreeColumns {
       mix(std::false_type{}, [](Frag f, int) { return f; });
     } else {
       mix(std::true_type{}, [&](Frag f, int t) {
+        if constexpr (KEYS == 2) {
+          words4 v = __builtin_bit_cast(words4, f);
+          tidy_values(v, s.len - p0 - value_key(t, qd), odd);
+          return __builtin_bit_cast(Frag, v);
+        }
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
           const bool none = p0 + value_key(t, qd) + e >= s.len, finite = fabsf(to_f32((T)f[e])) <= FLT_MAX;
@@ -430,7 +454,8 @@ __global__ __launch_bounds__(TREE_WAVES * WAVE, NC == 1 && sizeof(T) == 2 ? 2 : 
     float lt = sm_l[0][c * 16 + j];
 #pragma unroll
     for (int v = 1; v < NW; ++v) lt += sm_l[v][c * 16 + j];
-    const size_t head = (size_t)(s.row0 + x / G) * a.n_heads + w.g * G + x % G;
+    const int node = a.node_of(x);
+    const size_t head = (size_t)(s.row0 + node) * a.n_heads + w.g * G + x - node * G;
     const float inv = tree_inverse(lt);
     for (int dt = wave; dt < DT; dt += NW) {
       f32x4 v = sm_o[0][dt][lane];
