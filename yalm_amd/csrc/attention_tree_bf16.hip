@@ -152,22 +152,23 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
   }
   __syncthreads();
   if (!wide && half == 1) return;
+  // one step for all tiles and then the next, each without branches: this code runs once, and what it waits for most is itself
+  if (!wide) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float m2 = ml[(c * 2) * 256 + tid], l2 = ml[(c * 2 + 1) * 256 + tid], m = fmaxf(col.m[c], m2);
+      const float f1 = __builtin_amdgcn_exp2f(col.m[c] - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
+      col.m[c] = m;
+      col.l[c] = col.l[c] * f1 + l2 * f2;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) col.o[c][dt] = col.o[c][dt] * f1 + mo[(c * DT + dt) * 256 + tid] * f2;
+    }
+  }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const float m2 = wide ? -FLT_MAX : ml[(c * 2) * 256 + tid], l2 = wide ? 0.f : ml[(c * 2 + 1) * 256 + tid];
-    const float m = fmaxf(col.m[c], m2);
-    const float f1 = __builtin_amdgcn_exp2f(col.m[c] - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
-    const float lt = fold_column(col.l[c] * f1 + l2 * f2, [](float u, float v) { return u + v; });
+    const float lt = fold_column(col.l[c], [](float u, float v) { return u + v; });
     const int x = mine + c * step + j;
-    if (x >= cols) continue;
-    const int node = a.node_of(x);
-    const size_t head = (size_t)(s.row0 + node) * a.n_heads + w.g * G + x - node * G;
-    const float inv = tree_inverse(lt);
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      tree_store<bf16, HD>(a, head, w.split, dt * 16 + 4 * qd, wide ? col.o[c][dt] : col.o[c][dt] * f1 + mo[(c * DT + dt) * 256 + tid] * f2, inv);
-    if (a.n_splits > 1 && qd == 0)
-      *reinterpret_cast<float2*>(a.partial + (head * a.n_splits + w.split) * (HD + 2) + HD) = make_float2(m, lt);
+    if (x < cols) tree_leave<bf16, HD>(a, s, w, x, qd, col.m[c], lt, col.o[c]);
   }
 }
 

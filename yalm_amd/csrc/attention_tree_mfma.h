@@ -357,6 +357,34 @@ __device__ __forceinline__ void tree_store(const TreeArgs& a, size_t head, int s
 }
 __device__ __forceinline__ float tree_inverse(float l) { return l > 0.f ? 1.0f / l : l == l ? 0.f : l; }       // a sum that is no number stays one
 
+// All of column x's result, its sum folded: what lane (qd, j) holds of it.
+template <typename T, int HD>
+__device__ __forceinline__ void tree_leave(const TreeArgs& a, const TreeSeq& s, const TreeWork& w, int x, int qd, float m, float l,
+                                           const f32x4 (&o)[HD / 16]) {
+  const int G = a.n_heads / a.n_kv_heads, node = a.node_of(x);
+  const size_t head = (size_t)(s.row0 + node) * a.n_heads + w.g * G + x - node * G;
+  if (a.n_splits == 1) {
+    typedef __attribute__((ext_vector_type(4))) T out4;
+    T* to = (T*)a.out + head * HD + 4 * qd;
+    const float inv = tree_inverse(l);
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) {
+      out4 r4;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) r4[r] = from_f32<T>(o[dt][r] * inv);
+      *reinterpret_cast<out4*>(to + dt * 16) = r4;
+    }
+  } else {
+    float* to = a.partial + (head * a.n_splits + w.split) * (HD + 2);
+#pragma unroll
+    for (int dt = 0; dt < HD / 16; ++dt) {
+      *reinterpret_cast<float2*>(to + dt * 16 + 4 * qd) = make_float2(o[dt][0], o[dt][1]);
+      *reinterpret_cast<float2*>(to + dt * 16 + 4 * qd + 2) = make_float2(o[dt][2], o[dt][3]);
+    }
+    if (qd == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m, l);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Few columns (16 NC of them a workgroup): four waves take the pages of a split in turn, straight from memory into registers - a page
 // is one wave's, and its load instructions read 1 KB of consecutive bytes -, each with the keys of its next page in flight, and
