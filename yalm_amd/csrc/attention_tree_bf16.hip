@@ -20,6 +20,9 @@ int tree_columns(int B, int max_nodes, int n_heads, int n_kv_heads, int head_dim
 // columns, and leaves out those that the sequence does not fill.
 // ---------------------------------------------------------------------------
 template <int HD, int NC>
+constexpr int tree_merge_bytes() { return NC * (HD + 8) * 256; }
+
+template <int HD, int NC>
 __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int chunks, int wide_chunks) {
   typedef TreeColumns<bf16, HD, NC> C;
   static_assert(HD % 32 == 0, "pages in blocks");
@@ -164,18 +167,19 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
       for (int dt = 0; dt < DT; ++dt) col.o[c][dt] = col.o[c][dt] * f1 + mo[(c * DT + dt) * 256 + tid] * f2;
     }
   }
+  // behind what the second group left, which the other waves may still read
+  unsigned char* own = smem_raw + (wide ? 0 : tree_merge_bytes<HD, NC>()) + (wide ? wave + 4 * half : wave) * tree_leave_bytes<bf16, HD>();
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const float lt = fold_column(col.l[c], [](float u, float v) { return u + v; });
-    const int x = mine + c * step + j;
-    if (x < cols) tree_leave<bf16, HD>(a, s, w, x, qd, col.m[c], lt, col.o[c]);
+    tree_leave<bf16, HD>(a, s, w, mine + c * step, cols, lane, col.m[c], lt, col.o[c], own);
   }
 }
 
 template <int HD, int NC>
 int launch_lds(const TreeArgs& a, hipStream_t stream) {
-  constexpr int bytes = 8 * PAGE * HD * (int)sizeof(bf16), merge = NC * (HD / 16 * 16 + 8) * 256;
-  constexpr int lds = bytes > merge ? bytes : merge;
+  constexpr int lds = 8 * PAGE * HD * (int)sizeof(bf16);       // four pages of a head's keys and values
+  static_assert(lds >= tree_merge_bytes<HD, NC>() + 4 * tree_leave_bytes<bf16, HD>() && lds >= 8 * tree_leave_bytes<bf16, HD>(), "the results' places");
   auto kernel = &attn_tree_lds_kernel<HD, NC>;
   if (lds > 60 * 1024) {
     static LdsAllowance allowed;
