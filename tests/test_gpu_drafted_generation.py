@@ -252,3 +252,22 @@ def test_the_command_line_samples_and_drafts(folders, capsys):
     assert " ".join(map(str, want)) in run(*flags, "--draft", "4")
     with pytest.raises(SystemExit):
         main(args + ["--draft", "4", "-T", "16"])
+
+
+def test_settings_of_any_kind_of_number():
+    """Python's numbers, numpy's, arrays, tensors: one for all rows or one for each, the same tokens."""
+    from yalm_amd.sampling import Sampler
+    logits = torch.randn((3, 900), generator=torch.Generator().manual_seed(2)).to("cuda:0") * 3
+    sampler, ids, steps = Sampler(4), [0, 1, 2], [5, 6, 7]
+    plain = sampler.sample(logits, 0.75, ids, steps)
+    greedy = sampler.sample(logits, 0.0, ids, steps)
+    assert sampler.sample(logits, np.float32(0.75), ids, steps) == plain == sampler.sample(logits, torch.tensor(0.75), ids, steps)
+    assert sampler.sample(logits, np.float32(0.0), ids, steps) == greedy == sampler.sample(logits, 0, ids, steps)
+    want = sampler.sample(logits, 0.75, ids, steps, top_k=20, top_p=0.5)
+    for top_k in (np.int64(20), [20] * 3, np.full(3, 20), torch.full((3,), 20)):
+        for top_p in (np.float64(0.5), (0.5, 0.5, 0.5), np.full(3, 0.5, np.float32), torch.tensor(0.5)):
+            assert sampler.sample(logits, np.float32(0.75), ids, steps, top_k=top_k, top_p=top_p) == want
+    assert sampler.sample(logits, np.zeros(3), ids, steps) == greedy
+    for bad in (dict(top_k=[1, 2]), dict(top_p=1.5), dict(min_p=-0.1), dict(top_k=np.array([-1, 0, 0])), dict(top_p=float("nan"))):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            sampler.sample(logits, 1.0, ids, steps, **bad)

@@ -49,6 +49,11 @@ class Drawn:
         return self._list
 
 
+def _of_rows(value):
+    """Whether a setting is a sequence, one number a row (and no number of Python's, numpy's or torch's for all of them)."""
+    return hasattr(value, "__len__") and getattr(value, "ndim", 1) > 0
+
+
 class Sampler:
     HOST_BUFFERS = 4          # draws whose host copies may be unread at the same time
 
@@ -81,7 +86,7 @@ class Sampler:
         rows[0] = torch.tensor([uniform(self.seed, r, s) for r, s in zip(request_ids, steps)], dtype=torch.float32)
         for i, (name, value) in enumerate(settings.items()):
             whole = name == "top_k"
-            if isinstance(value, (int, float)):
+            if not _of_rows(value):
                 value = [value] * R
             value = [int(v) if whole else float(v) for v in value]
             if len(value) != R:
@@ -107,7 +112,7 @@ class Sampler:
         while the host reads them a step later."""
         R = logits.shape[0]
         settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
-        filtered = settings != {"temperature": temperature, "top_k": 0, "top_p": 1.0, "min_p": 0.0} or not isinstance(temperature, (int, float))
+        filtered = any(_of_rows(v) for v in settings.values()) or (top_k, top_p, min_p) != (0, 1.0, 0.0)
         out = torch.empty(R, dtype=torch.int32, device=logits.device)
         host, host_u, landed = self._host_buffers(R)
         if filtered:
