@@ -271,3 +271,14 @@ def test_settings_of_any_kind_of_number():
     for bad in (dict(top_k=[1, 2]), dict(top_p=1.5), dict(min_p=-0.1), dict(top_k=np.array([-1, 0, 0])), dict(top_p=float("nan"))):
         with pytest.raises(ValueError, match=next(iter(bad))):
             sampler.sample(logits, 1.0, ids, steps, **bad)
+
+
+def test_guesses_deeper_than_the_window(folders):
+    from yalm_amd import generate, generate_drafted
+    engine = engine_of(folders, "tiny_mistral", torch.float32, max_draft=40)
+    assert engine.max_draft_depth == tiny_configs.ALL["tiny_mistral"]["sliding_window"] < 40
+    prompt = [5, 9] * 20
+    chain = lambda history, n: ((history[-1:] + prompt * 2)[:n], list(range(-1, n - 1)))  # noqa: E731
+    want = generate(engine, [prompt], max_new_tokens=60, stop_ids=[])
+    assert generate_drafted(engine, [prompt], max_new_tokens=60, stop_ids=[], max_nodes=40, guess=chain) == want
+    assert generate_drafted(engine, [prompt], max_new_tokens=60, stop_ids=[], max_nodes=40) == want

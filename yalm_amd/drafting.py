@@ -103,8 +103,8 @@ def generate_drafted(engine, prompts, max_new_tokens=256, temperature=0.0, seed=
                 trees = []
                 for i, s in live:
                     history = list(prompts[i]) + results[i]
-                    # no deeper than the request's tokens and the context go, and no wider than the places behind its tokens
-                    left = min(max_new_tokens - len(results[i]), max_len - len(history))
+                    # no deeper than the request's tokens, the context and a window go, and no wider than the places behind its tokens
+                    left = min(max_new_tokens - len(results[i]), max_len - len(history), engine.max_draft_depth)
                     tokens, parents = guess(history, max(1, min(max_nodes, engine.cache.max_seq_len - engine.length(s) if not engine.cache.unbounded
                                                                 else max_nodes)))
                     trees.append(_shallow(tokens, parents, left))

@@ -100,6 +100,8 @@ class Engine:
                                   self.device, n_slots=max_batch, max_draft=min(int(max_draft), kernels.MAX_TREE_NODES) if model.takes_drafts() else 0)
         windowed = any(g.window > 0 for g in self.cache.kv_groups)
         self.max_draft = min(int(max_draft), kernels.MAX_TREE_NODES) if windowed else kernels.MAX_TREE_NODES
+        # a node sees its root: depths stay below the narrowest window
+        self.max_draft_depth = min([g.window for g in self.cache.kv_groups if g.window > 0] + [kernels.MAX_TREE_NODES])
         self._drafted = {}                              # slot -> (tokens held before, the parents of its drafted tokens)
         n_positions = model.spec.max_positions if self.cache.unbounded else \
             min(model.spec.max_positions, self.cache.max_seq_len)
@@ -318,9 +320,8 @@ class Engine:
             row += n
             trees.append(up)
             depths.append(depth)
-        narrowest = min([g.window for g in self.cache.kv_groups if g.window] + [1 << 30])
-        if max(d for ds in depths for d in ds) >= narrowest:
-            raise StepError("a tree as deep as the window of %d positions is refused" % narrowest)
+        if max(d for ds in depths for d in ds) >= self.max_draft_depth:
+            raise StepError("a tree as deep as the window of %d positions is refused" % self.max_draft_depth)
         max_pos = max(s + max(d) for s, d in zip(starts, depths))
         new_lens = self._extend(slots, n_tok, max_pos)
         cu = np.zeros(B + 1, dtype=np.int32)
