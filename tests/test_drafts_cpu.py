@@ -20,6 +20,38 @@ def test_tensors_that_are_not_on_the_gpu_are_refused():
                           torch.zeros((1, 1), dtype=torch.int64), torch.zeros((1, 16)), torch.zeros(0), 1, 1, 16, 0, 1, 1)
 
 
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    class OnSecond(torch.Tensor):                      # a tensor that says it lies on the second GPU
+        is_cuda = True
+
+        def get_device(self):
+            return 1
+
+    def on_second(*a, **kw):
+        return torch.zeros(*a, **kw).as_subclass(OnSecond)
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    i, cu, i2 = on_second(1, dtype=torch.int32), on_second(2, dtype=torch.int32), on_second((1, 1), dtype=torch.int32)
+    k, v = on_second((1, 2, 1, 64, 16)), on_second((1, 2, 1, 16, 64))
+    with pytest.raises(RuntimeError, match="device 1"):
+        kernels.sample_filtered(on_second((2, 8)), on_second(2), cu)
+    with pytest.raises(RuntimeError, match="device 1"):
+        kernels.copy_pages(k, v, i, i)
+    with pytest.raises(RuntimeError, match="device 1"):
+        kernels.compact_lines(k, v, i2, 1, i, i, cu, i, 1)
+    with pytest.raises(RuntimeError, match="device 1"):
+        kernels.attn_tree(on_second((1, 16)), k[0], v[0], i2, 1, i, i, cu, on_second((1, 1), dtype=torch.int64), on_second((1, 16)), on_second(0), 1, 1, 16, 0,
+                          1, 1)
+
+
+def test_the_command_line_s_settings_are_checked():
+    from yalm_amd import cli
+    for bad in (["--draft", "256"], ["--draft", "-1"], ["--top-p", "1.5"], ["--min-p", "-1"], ["--top-k", "-2"], ["--samples", "0"], ["--draft", "2", "--samples", "2"]):
+        with pytest.raises(SystemExit):
+            cli.parse_args(["folder", "-i", "text"] + bad)
+    assert cli.parse_args(["folder", "-i", "text", "--draft", "255"])["draft"] == 255
+
+
 def test_shapes_that_say_nothing_are_refused():
     with pytest.raises(ValueError, match="vocabulary"):
         kernels.sample_filtered(torch.zeros(8), None, None)

@@ -90,8 +90,8 @@ def parse_args(argv):
         else:
             error_usage("unknown option %s" % flag)
         i += 2
-    if a["top_k"] < 0 or not 0 <= a["top_p"] <= 1 or not 0 <= a["min_p"] <= 1 or a["samples"] < 1 or a["draft"] < 0:
-        error_usage("--top-k and --draft are 0 or more, --top-p and --min-p between 0 and 1, --samples 1 or more")
+    if a["top_k"] < 0 or not 0 <= a["top_p"] <= 1 or not 0 <= a["min_p"] <= 1 or a["samples"] < 1 or not 0 <= a["draft"] <= 255:
+        error_usage("--top-k is 0 or more, --draft between 0 and 255, --top-p and --min-p between 0 and 1, --samples 1 or more")
     if a["draft"] and a["samples"] > 1:
         error_usage("--draft and --samples do not go together")
     if a["dtype"] not in ("bfloat16", "float32"):

@@ -73,6 +73,12 @@ def _need(t, name, dtype=None, shape=None):
     return t.data_ptr()
 
 
+def _on_current(t, name):
+    """Refuses a tensor of another device than the current one, on whose stream the launch goes."""
+    if t.get_device() != torch.cuda.current_device():
+        raise RuntimeError("%s lies on device %d, the current one is %d (torch.cuda.device says which)" % (name, t.get_device(), torch.cuda.current_device()))
+
+
 def _rows(t, name, T, width):
     """(address, elements from row to row) of a float32 [T, width] on the device whose rows may be parts of wider rows."""
     if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.dim() != 2 or tuple(t.shape) != (T, width) \
@@ -943,6 +949,7 @@ def attn_tree(q, k_pages, v_pages, block_table, ring_pages, seq_slot, seq_len, c
         raise ValueError("ring_pages %d does not fit the block table (%d columns)" % (ring_pages, stride))
     p_ss = _need(seq_slot, "seq_slot", torch.int32, (None,))
     B = seq_slot.shape[0]
+    _on_current(q, "q")
     p_m = _need(mask, "mask", torch.int64, (T, None))
     words = mask.shape[1]
     if not 1 <= max_nodes <= MAX_TREE_NODES or words < 1 or max_nodes > 64 * words:
@@ -1997,7 +2004,8 @@ def sample_filtered(logits, u, out, temperature=None, top_k=None, top_p=None, mi
     if V < 1:
         raise ValueError("sample_filtered needs a vocabulary")
     n = (R,)
-    p_ws = None
+    p_logits, p_ws = _need(logits, "logits", torch.float32), None
+    _on_current(logits, "logits")
     if workspace is not None:
         p_ws = _need(workspace, "workspace", torch.int32)
         if workspace.numel() < sample_filtered_workspace(R, V):
@@ -2005,7 +2013,7 @@ def sample_filtered(logits, u, out, temperature=None, top_k=None, top_p=None, mi
         if p_ws % 16 or workspace.numel() == 0:
             p_ws = None                       # a part of a buffer that the kernels' 16-byte loads cannot take: as without one
     library.check(library.lib().yalm_sample_filtered(
-        _need(logits, "logits", torch.float32), _need(u, "u", torch.float32, n), _opt(temperature, "temperature", torch.float32, n),
+        p_logits, _need(u, "u", torch.float32, n), _opt(temperature, "temperature", torch.float32, n),
         _opt(top_k, "top_k", torch.int32, n), _opt(top_p, "top_p", torch.float32, n), _opt(min_p, "min_p", torch.float32, n),
         _need(out, "out", torch.int32, n), _opt(prob, "prob", torch.float32, n), p_ws, R, V, _stream()), "sample_filtered")
     return out
@@ -2016,6 +2024,7 @@ def copy_pages(k_pages, v_pages, src, dst):
     dst[i] (int32 [n] each, on the device).  No page may be the source of one pair and the destination of another; of several copies to one
     page the last one stands, and a number that is no page is passed over."""
     p_k = _need(k_pages, "k_pages")
+    _on_current(k_pages, "k_pages")
     p_v = None
     if k_pages.dim() < 2:
         raise ValueError("k_pages: [lines, pages, ...] is expected, got %s" % list(k_pages.shape))
@@ -2042,6 +2051,7 @@ def compact_lines(k_pages, v_pages, block_table, ring_pages, seq_slot, seq_start
     dt = k_pages.dtype
     L, n_pages, H, _, hd = k_pages.shape
     p_k = _need(k_pages, "k_pages", dt, (L, n_pages, H, PAGE, hd))
+    _on_current(k_pages, "k_pages")
     p_v = _need(v_pages, "v_pages", dt, (L, n_pages, H, hd, PAGE))
     p_t = _need(block_table, "block_table", torch.int32, (None, None))
     n_slots, stride = block_table.shape
