@@ -27,7 +27,8 @@ __device__ __forceinline__ int sequence_of(const int* cu, int B, int r) {
 
 // ---------------------------------------------------------------------------
 // Every head size and type, in float32 arithmetic: a wave a (row, head), 64 keys at a time, a lane a key for the scores and a
-// lane an output element for the mix.  For the shapes that the matrix cores' kernel does not take.
+// lane an output element for the mix.  For the shapes that the matrix cores' kernel does not take; every row reads its sequence's keys
+// by itself, which is what bounds it (16 nodes of 32 heads of 128 behind 3,056 tokens, bfloat16: 1,344 us, where that kernel takes 15).
 // ---------------------------------------------------------------------------
 constexpr int MAX_HD = 1024;
 
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(WAVE) void attn_tree_simple_kernel(TreeArgs a) {
 
 // ---------------------------------------------------------------------------
 // The splits' parts [T, n_heads, n_splits, hd + 2] = (sum[hd], maximum as an exponent of 2, denominator), merged in one order: a
-// wave a (row, head).
+// wave a (row, head).  12 splits of 16 rows of 32 heads of 128 4.0 us, 16 of 61 rows 5.4 (16 MB from the cache, 3 TB/s): a launch and two trips to memory.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void attn_tree_merge_kernel(TreeArgs a) {

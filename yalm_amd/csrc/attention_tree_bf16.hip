@@ -3,18 +3,23 @@
 
 namespace {
 
-// The columns that a workgroup takes.
+// The columns that a workgroup takes: no more tiles than the step fills.  More than 32 go over LDS, where a page is read once for all of
+// them (61 nodes, 244 columns, behind 28,000 tokens: 47.5 us, in 32s from registers 65 with the splits that suit those; 64 sequences of 40 nodes 157, 225).  More than
+// 128 go in one workgroup as soon as the halves would not all run at once (61 nodes behind 2,000 tokens, 8 KV heads, no splits: 18 sequences 74 us, in halves 92; 28
+// 81 and 100), and in halves as long as they do (16 sequences 48 us, in one 74; one sequence of 28,000 in 16 splits 47.5, in one 71).
 int tree_columns(int B, int max_nodes, int n_heads, int n_kv_heads, int head_dim) {
   const long cols = (long)max_nodes * (n_heads / n_kv_heads);
   if (cols <= 16) return 16;
   if (cols <= 32 || head_dim % 32 != 0) return 32;
   if (cols <= 64) return 64;
-  return cols > 128 && 2l * B * n_kv_heads >= compute_units() ? 256 : 128;
+  return cols > 128 && 2l * B * n_kv_heads > compute_units() ? 256 : 128;
 }
 
 // ---------------------------------------------------------------------------
 // More columns: eight waves share a run of pages, which go from memory straight into LDS two at a time (pages in blocks: a fragment is 1 KB
-// of consecutive bytes), the next two in flight while these are multiplied.  With up to 64 NC columns
+// of consecutive bytes), the next two in flight while these are multiplied.  A round of two pages against 128 columns of 128 elements takes 2.0 us: its
+// softmax (vector units 47 %) and its products (matrix cores 28 %) follow each other in a wave, and with 128 KB of pages a compute unit holds one workgroup.
+// One sequence of 28,000 tokens and 61 nodes 46 us (2.5 TB/s, 600 TFLOP/s), 64 of up to 3,041 and 40 nodes 157 (3.6 TB/s).  With up to 64 NC columns
 // two groups of four waves take a page each and the second hands its results to the first at the end; with more (`wide`, up
 // to 128 NC) all eight waves split the columns and take both pages.  A wave has the tiles wave, wave + 4 (wide: + 8), ... of 16
 // columns, and leaves out those that the sequence does not fill.

@@ -903,14 +903,18 @@ MAX_TREE_NODES = 256             # drafted tokens of a sequence that attn_tree t
 
 def attn_tree_splits(n_seqs, max_nodes, max_len, n_heads, n_kv_heads, head_dim, dtype, window=0):
     """Into how many pieces attn_tree should cut the keys of a sequence, so that its workgroups fill the chip: of steps of n_seqs sequences
-    of up to max_len tokens, the drafted ones (up to max_nodes) among them."""
+    of up to max_len tokens, the drafted ones (up to max_nodes) among them.
+
+    As many as run at once, of four pages and more each.  In bfloat16, 32 heads in 8 groups of 128, us: one sequence of 28,000 tokens and 61 nodes in 8, 16 and 32 pieces
+    72, 47.5 and 56; of 3,056 and 16 nodes in 8, 12 and 16 16.1, 15.5 and 16.2; 8 sequences of 2,000 and 61 nodes in 1, 2 and 4 47, 42 and 50; where whole
+    sequences fill the chip a second piece costs its merge and more (16 of 2,000 and 61 nodes 48 and 75, 64 of 209 and 16 nodes 25 and 61)."""
     if head_dim % 16 or head_dim > 128 or FORCE_SIMPLE:
         return 1
-    cols = max_nodes * (n_heads // n_kv_heads)
+    cols = max_nodes * (n_heads // n_kv_heads)      # a workgroup's share of them: as the kernels cut them
     if dtype == torch.float32:
         tile, resident = (32 if cols > 16 and head_dim <= 96 else 16), 256
     elif cols > 32 and head_dim % 32 == 0:
-        tile, resident = (64 if cols <= 64 else 256 if cols > 128 and 2 * n_seqs * n_kv_heads >= 256 else 128), 256
+        tile, resident = (64 if cols <= 64 else 256 if cols > 128 and 2 * n_seqs * n_kv_heads > 256 else 128), 256
     else:
         tile, resident = (32, 256) if cols > 16 else (16, 512)
     pages = (max_len + PAGE - 1) // PAGE
