@@ -106,13 +106,16 @@ __global__ __launch_bounds__(512, 1) void attn_tree_lds_kernel(TreeArgs a, int c
         // what they are is not always 0); the latter are read again behind the walk, for the columns that see them.
         if constexpr (EDGE) {
           bool mine_odd = false;
-          const int here = from_here(tid);
-          if (first + half < pages.end) {
-            bf16* vs = reinterpret_cast<bf16*>(smem_raw) + (size_t)((buf * 2 + half) * 2 + 1) * TILE;
-            const int left = s.len - (first + half) * PAGE;
+          const int here = from_here(threadIdx.x);
+#pragma unroll 1
+          for (int which = 0; which < 2; ++which) {
+            if (first + which >= pages.end || !col.at_edge(s, first + which)) continue;
+            bf16* vs = reinterpret_cast<bf16*>(smem_raw) + (size_t)((buf * 2 + which) * 2 + 1) * TILE;
+            const int left = s.len - (first + which) * PAGE;
 #pragma unroll
-            for (int p = 0; p < NLOAD; ++p) {
-              const int piece = here + p * 256, key = piece % 64 / 16 * 8 + piece / (4 * HD) * 32;      // eight keys of an element
+            for (int p = 0; p < (NLOAD + 1) / 2; ++p) {
+              const int piece = here + p * 512, key = piece % 64 / 16 * 8 + piece / (4 * HD) * 32;      // eight keys of an element
+              if (NLOAD % 2 != 0 && piece >= TILE / 8) continue;
               words4 v = *reinterpret_cast<const words4*>(vs + piece * 8);
               if (tidy_values(v, left - key, mine_odd)) *reinterpret_cast<words4*>(vs + piece * 8) = v;
             }
