@@ -63,6 +63,34 @@ def test_shapes_that_say_nothing_are_refused():
         kernels.attn_tree(None, None, None, None, 1, None, None, None, None, None, None, 3, 2, 64, 0, 1, 1)
 
 
+@pytest.mark.parametrize("wrong", [dict(n_heads=3), dict(head_dim=0), dict(head_dim=2048), dict(ring=0), dict(ring=9), dict(n_slots=0), dict(words=0), dict(n_splits=0),
+                                   dict(max_nodes=0), dict(max_nodes=257), dict(n_pages=0), dict(layout=1, head_dim=48), dict(dtype=7), dict(n_heads=65536, n_kv=1)])
+def test_the_library_s_entry_refuses_numbers_that_name_no_step(wrong):
+    """The C entry by itself, without memory behind its pointers: it answers before it would launch."""
+    from yalm_amd.ops import library
+    s = {**dict(T=5, B=1, n_heads=4, n_kv=2, head_dim=64, n_splits=1, max_nodes=5, n_pages=3, layout=1, dtype=0, ring=2, stride=8, n_slots=2, words=1), **wrong}
+    code = library.lib().yalm_attn_tree(None, None, None, None, s["stride"], s["n_slots"], s["ring"], None, None, None, None, s["words"], None, None, None, s["T"], s["B"],
+                                        s["n_heads"], s["n_kv"], s["head_dim"], 0, s["n_splits"], s["max_nodes"], s["n_pages"], s["layout"], s["dtype"], 0, None,
+                                        None)
+    assert code != 0
+    with pytest.raises(Exception):
+        library.check(code, "attn_tree")
+
+
+def test_the_library_s_other_entries_refuse_too():
+    from yalm_amd.ops import library
+    lib = library.lib()
+    assert lib.yalm_sample_filtered(None, None, None, None, None, None, None, None, None, 2, 0, None) != 0
+    assert lib.yalm_sample_filtered(None, None, None, None, None, None, None, None, 8, 2, 100, None) != 0       # a workspace off 16 bytes
+    assert lib.yalm_sample_filtered(None, None, None, None, None, None, None, None, None, 0, 100, None) == 0    # no rows
+    assert lib.yalm_copy_blocks(None, None, 2, 3, 64, None, None, 1, None) != 0
+    assert lib.yalm_copy_blocks(None, None, 2, 3, 64, None, None, 0, None) == 0
+    for kw in (dict(ring=0), dict(ring=5), dict(slots=0), dict(lines=65536), dict(pages=0), dict(layout=1, hd=48), dict(B=65536)):
+        s = {**dict(ring=2, slots=2, lines=2, pages=3, layout=1, hd=64, B=1), **kw}
+        assert lib.yalm_compact_lines(None, None, None, 4, s["slots"], s["ring"], None, None, None, None, s["B"], 1, 1, s["lines"], s["pages"], 1, s["hd"], s["layout"], 0,
+                                      None) != 0, kw
+
+
 def test_workspace_sizes():
     assert kernels.attn_tree_workspace_floats(7, 4, 64, 1) == 0
     assert kernels.attn_tree_workspace_floats(7, 4, 64, 3) == 7 * 4 * 3 * 66
