@@ -54,6 +54,10 @@ def _of_rows(value):
     return hasattr(value, "__len__") and getattr(value, "ndim", 1) > 0
 
 
+# what each setting of a draw may be
+SETTINGS = {"temperature": (0.0, math.inf), "top_k": (0, 2 ** 31 - 1), "top_p": (0.0, 1.0), "min_p": (0.0, 1.0)}
+
+
 class Sampler:
     HOST_BUFFERS = 4          # draws whose host copies may be unread at the same time
 
@@ -64,38 +68,46 @@ class Sampler:
         self._turn = 0
 
     def _host_buffers(self, R):
-        """The next pinned pair in turn: int32 for the tokens on their way back, float32 for the
-        uniform numbers and the rows' settings on their way out, and the event behind the draw that used them last."""
-        if len(self._host) < self.HOST_BUFFERS:
+        """The pinned pair of this turn: int32 for the tokens on their way back, float32 for the
+        uniform numbers and the rows' settings on their way out, and the event behind the draw that used them last.
+        A draw that fails behind this leaves the turn where it was, and the next one takes the same pair."""
+        turn = self._turn % self.HOST_BUFFERS
+        if turn == len(self._host):
             n = max(R, 64)
             self._host.append([torch.empty(n, dtype=torch.int32, pin_memory=True),
                                torch.empty(5 * n, dtype=torch.float32, pin_memory=True), torch.cuda.Event()])
             return self._host[-1]
-        entry = self._host[self._turn % self.HOST_BUFFERS]
+        entry = self._host[turn]
         entry[2].synchronize()
         if entry[0].shape[0] < R:
             entry[0] = torch.empty(R, dtype=torch.int32, pin_memory=True)
             entry[1] = torch.empty(5 * R, dtype=torch.float32, pin_memory=True)
         return entry
 
+    @staticmethod
+    def _checked(settings, R):
+        """The settings of a draw under filters, each a number for all rows or a list of one for each, after the checks."""
+        out = {}
+        for name, value in settings.items():
+            of_rows = _of_rows(value)
+            values = [int(v) if name == "top_k" else float(v) for v in (value if of_rows else [value])]
+            if of_rows and len(values) != R:
+                raise ValueError("%s: %d settings for %d rows" % (name, len(values), R))
+            low, high = SETTINGS[name]
+            if not all(low <= v <= high for v in values):
+                raise ValueError("%s: %s is not between %s and %s" % (name, values, low, high))
+            out[name] = values if of_rows else values[0]
+        return out
+
     def _filtered(self, logits, out, host, settings, request_ids, steps):
-        """sample_filtered with the rows' numbers and settings uploaded together, and a workspace kept from draw to draw (draws of one
+        """sample_filtered with the rows' numbers and settings (_checked) uploaded together, and a workspace kept from draw to draw (draws of one
         sampler follow each other on one stream)."""
         R, V = logits.shape
         rows = host[:5 * R].view(5, R)
         rows[0] = torch.tensor([uniform(self.seed, r, s) for r, s in zip(request_ids, steps)], dtype=torch.float32)
-        for i, (name, value) in enumerate(settings.items()):
-            whole = name == "top_k"
-            if not _of_rows(value):
-                value = [value] * R
-            value = [int(v) if whole else float(v) for v in value]
-            if len(value) != R:
-                raise ValueError("%s: %d settings for %d rows" % (name, len(value), R))
-            low, high = {"temperature": (0.0, math.inf), "top_k": (0, 2 ** 31 - 1), "top_p": (0.0, 1.0), "min_p": (0.0, 1.0)}[name]
-            if not all(low <= v <= high for v in value):
-                raise ValueError("%s: %s is not between %s and %s" % (name, value, low, high))
-            at = rows[1 + i]
-            (at.view(torch.int32) if whole else at).copy_(torch.tensor(value, dtype=torch.int32 if whole else torch.float32))
+        for at, (name, value) in zip(rows[1:], settings.items()):
+            dtype = torch.int32 if name == "top_k" else torch.float32
+            at.view(dtype).copy_(torch.tensor(value, dtype=dtype))
         dev = torch.empty((5, R), dtype=torch.float32, device=logits.device)
         dev.copy_(rows, non_blocking=True)                # from pinned memory: the host does not wait for the queue
         need = kernels.sample_filtered_workspace(R, V)
@@ -113,6 +125,8 @@ class Sampler:
         R = logits.shape[0]
         settings = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
         filtered = any(_of_rows(v) for v in settings.values()) or (top_k, top_p, min_p) != (0, 1.0, 0.0)
+        if filtered:
+            settings = self._checked(settings, R)         # in front of the buffers: a refused draw takes none
         out = torch.empty(R, dtype=torch.int32, device=logits.device)
         host, host_u, landed = self._host_buffers(R)
         if filtered:
