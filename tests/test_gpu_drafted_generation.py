@@ -282,3 +282,39 @@ def test_guesses_deeper_than_the_window(folders):
     want = generate(engine, [prompt], max_new_tokens=60, stop_ids=[])
     assert generate_drafted(engine, [prompt], max_new_tokens=60, stop_ids=[], max_nodes=40, guess=chain) == want
     assert generate_drafted(engine, [prompt], max_new_tokens=60, stop_ids=[], max_nodes=40) == want
+
+
+def test_draws_of_one_sampler_on_two_streams():
+    """Draws under filters that may run at the same time: the tokens of draws one behind the other."""
+    from yalm_amd.sampling import Sampler
+    g = torch.Generator().manual_seed(6)
+    logits = [(torch.randn((24, 50000), generator=g) * 2).to("cuda:0") for _ in range(4)]
+    ids, how = list(range(24)), dict(top_p=0.9)
+    sampler = Sampler(9)
+    want = [sampler.sample(x, 0.8, ids, [i] * 24, top_k=[0, 40] * 12, **how) for i, x in enumerate(logits)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        drawn = []
+        for i, x in enumerate(logits):
+            with torch.cuda.stream(streams[i % 2]):
+                drawn.append(sampler.draw(x, 0.8, ids, [i] * 24, top_k=[0, 40] * 12, **how))
+        assert [d.tolist() for d in drawn] == want
+
+
+def test_draws_behind_refused_ones():
+    """A refused draw, then more draws than there are buffers, each read only when no more may be unread."""
+    from yalm_amd.sampling import Sampler
+    logits = [torch.randn((3, 700), generator=torch.Generator().manual_seed(i)).to("cuda:0") for i in range(9)]
+    ids = [0, 1, 2]
+    want = [Sampler(5).sample(x, 0.9, ids, [i] * 3, top_p=0.8) for i, x in enumerate(logits)]
+    for refusals in (1, 2, 3):
+        s, waiting, got = Sampler(5), [], []
+        for i, x in enumerate(logits):
+            if i < refusals:
+                with pytest.raises(ValueError):
+                    s.draw(x, 0.9, ids, [i] * 3, top_p=1.5)
+            waiting.append(s.draw(x, 0.9, ids, [i] * 3, top_p=0.8))
+            if len(waiting) == Sampler.HOST_BUFFERS:
+                got.append(waiting.pop(0).tolist())
+        assert got + [d.tolist() for d in waiting] == want

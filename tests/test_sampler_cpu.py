@@ -80,3 +80,11 @@ def test_draws_behind_a_failed_one_are_their_own(stand_in, how):
             read_late(s, how)
         stand_in["fail"] = False
         assert read_late(s, how) == [[before + i] * 2 for i in range(8)]
+
+
+def test_draws_under_filters_have_workspaces_of_their_own(stand_in):
+    """Draws on several streams may run at the same time: as long as one's workspace lives, no other draw is given it."""
+    s = Sampler(3)
+    draws = [s.draw(torch.zeros((2, 5)), 0.7, [0, 1], [i, i], top_p=0.9) for i in range(3)]
+    assert len({w.data_ptr() for w in stand_in["workspaces"]}) == 3 and all(w.numel() >= 12 for w in stand_in["workspaces"])
+    assert [d.tolist() for d in draws] == [[i, i] for i in range(3)]

@@ -63,7 +63,6 @@ class Sampler:
 
     def __init__(self, seed=0):
         self.seed = int(seed)
-        self._scratch = None      # workspace of the draws under filters
         self._host = []           # pinned buffers and the events after the copies into them, used in turn
         self._turn = 0
 
@@ -100,8 +99,8 @@ class Sampler:
         return out
 
     def _filtered(self, logits, out, host, settings, request_ids, steps):
-        """sample_filtered with the rows' numbers and settings (_checked) uploaded together, and a workspace kept from draw to draw (draws of one
-        sampler follow each other on one stream)."""
+        """sample_filtered with the rows' numbers and settings (_checked) uploaded together.  The workspace is the current stream's own memory
+        until the draw has run (the allocator hands it on within the stream only): draws on several streams may run at the same time."""
         R, V = logits.shape
         rows = host[:5 * R].view(5, R)
         rows[0] = torch.tensor([uniform(self.seed, r, s) for r, s in zip(request_ids, steps)], dtype=torch.float32)
@@ -110,11 +109,9 @@ class Sampler:
             at.view(dtype).copy_(torch.tensor(value, dtype=dtype))
         dev = torch.empty((5, R), dtype=torch.float32, device=logits.device)
         dev.copy_(rows, non_blocking=True)                # from pinned memory: the host does not wait for the queue
-        need = kernels.sample_filtered_workspace(R, V)
-        if self._scratch is None or self._scratch.numel() < need or self._scratch.device != logits.device:
-            self._scratch = torch.empty(max(need, 1), dtype=torch.int32, device=logits.device)
+        workspace = torch.empty(kernels.sample_filtered_workspace(R, V), dtype=torch.int32, device=logits.device)
         kernels.sample_filtered(logits, dev[0], out, temperature=dev[1], top_k=dev[2].view(torch.int32), top_p=dev[3], min_p=dev[4],
-                                workspace=self._scratch)
+                                workspace=workspace)
 
     def draw(self, logits, temperature, request_ids, steps, top_k=0, top_p=1.0, min_p=0.0):
         """One token for each row of logits [R, vocab] (device, float32); temperature 0 is argmax.  top_k (0: off), top_p (1: off) and
