@@ -217,3 +217,117 @@ def test_command_line_settings():
     for bad in (["--top-k", "-1"], ["--top-p", "1.2"], ["--min-p", "-0.1"], ["--samples", "0"], ["--draft", "-2"], ["--draft", "2", "--samples", "2"]):
         with pytest.raises(SystemExit):
             parse_args(["folder", "--tokens", "1,2"] + bad)
+
+
+# ------------------------------------------------------------------------------------------------ rings and what their windows see
+def _windows(max_tokens, max_seq_len, windows=(100,), n_slots=4, **kw):
+    from yalm_amd.cache import CacheManager, KVRequest
+    return CacheManager({i: KVRequest(1, 4, w) for i, w in enumerate(windows)}, max_tokens, max_seq_len, torch.float32, "cpu", n_slots=n_slots, **kw)
+
+
+class Lines:
+    """What a ring's pages hold, written as the kernels write them: whole prompts by pages, later tokens one place each."""
+
+    def __init__(self, c):
+        self.c, self.at = c, {}
+
+    def grow(self, slot, n):
+        old = self.c.seq_len[slot]
+        (new,) = self.c.extend([slot], [n])
+        for i, g in enumerate(self.c.kv_groups):
+            for pos in range(old, new):
+                if old > 0 or pos // 64 > (new - 1) // 64 - g.ring_pages:
+                    page = int(g.table_host[slot, pos // 64 % g.ring_pages])
+                    assert 0 <= page < g.n_pages
+                    self.at[i, page, pos % 64] = (slot, pos)
+        return old, new
+
+    def check(self, slot, old, new):
+        """Every key that the tokens at old ... new - 1 see is held, the drafted ones themselves too."""
+        for i, g in enumerate(self.c.kv_groups):
+            for pos in range(max(0, old - g.window + 1), new):
+                assert self.at[i, int(g.table_host[slot, pos // 64 % g.ring_pages]), pos % 64] == (slot, pos), (i, pos, old, new)
+
+
+@pytest.mark.parametrize("windows,max_tokens,max_seq_len,max_draft,refuses",
+                         [((4096,), 256, 8192, 32, True), ((1024,), 4096, 1024, 8, False), ((1024,), 1024, 1024, 8, True), ((100,), 128, 400, 70, True),
+                          ((100, 300), 256, 1000, 9, True), ((62,), 64, 4000, 0, True), ((100,), 1024, 1024, 70, False), ((64,), 320, 64, 17, False)])
+def test_drafted_tokens_never_lie_on_keys_that_a_window_sees(windows, max_tokens, max_seq_len, max_draft, refuses):
+    """Prompts and trees of any size: what is not refused keeps all that it sees, and a refusal changes nothing."""
+    from yalm_amd.cache import CacheFull
+    rng = __import__("random").Random(max_tokens + max_draft)
+    went_on = refused = 0
+    for prompt in (1, 30, 63, 64, 65, 90, 150, 250, 1010):
+        c = _windows(max_tokens, max_seq_len, windows, max_draft=max_draft)
+        lines = Lines(c)
+        (s,) = c.acquire(1)
+        if prompt > max_seq_len:
+            continue
+        lines.grow(s, prompt)
+        for _ in range(300):
+            n = rng.randint(1, max(1, max_draft)) if rng.random() < 0.5 else 1
+            before = (c.seq_len[s], [g.pool.n_free for g in c.kv_groups], [g.table_host.copy() for g in c.kv_groups], c.room(s))
+            if before[0] + n > max_seq_len + max_draft:
+                break
+            try:
+                lines.check(s, *lines.grow(s, n))
+                went_on += 1
+                assert n <= before[3]
+            except CacheFull:
+                refused += 1
+                assert before[:2] == (c.seq_len[s], [g.pool.n_free for g in c.kv_groups]) and all((a == g.table_host).all() for a, g in zip(before[2], c.kv_groups))
+                assert n > before[3]
+                if before[3] < 1:
+                    break
+                continue
+            c.cut([s], [before[0] + rng.randint(1, n)])
+        c.release([s])
+        assert all(g.pool.n_free == g.n_pages for g in c.kv_groups)
+    assert went_on > 40 and (refused > 0) == refuses
+
+
+def test_rings_have_room_for_drafts_up_to_the_end_of_the_context():
+    c = _windows(4096, 1024, (1024,), max_draft=8)
+    assert c.kv_groups[0].ring_pages == 17
+    (s,) = c.acquire(1)
+    c.extend([s], [1019])
+    assert c.extend([s], [8]) == [1027] and c.kv_groups[0].pool.n_free == 64 - 17
+    assert _windows(4096, 1024, (1024,)).kv_groups[0].ring_pages == 16           # without drafts no sequence is longer
+    assert _windows(4096, 64, (62,), longest=500).kv_groups[0].ring_pages == 2   # a text that runs past the model's positions
+    assert _windows(64, 64, (62,), longest=500).kv_groups[0].ring_pages == 1
+
+
+def test_a_sequence_that_outgrows_a_small_cache_is_refused():
+    """The window is wider than all pages together: the prompt itself may be longer (its own keys are staged), but nothing goes on where a
+    key in sight is gone."""
+    from yalm_amd.cache import CacheFull
+    c = _windows(256, 8192, (4096,))
+    a, b = c.acquire(2)
+    c.extend([a], [256])
+    with pytest.raises(CacheFull, match="window"):
+        c.extend([a], [1])
+    assert c.seq_len[a] == 256 and c.room(a) == 0
+    c.release([a])
+    c.extend([b], [300])
+    with pytest.raises(CacheFull, match="window"):
+        c.extend([b], [1])
+    c.release([b])
+    (a,) = c.acquire(1)                                # nothing of the last sequence sticks to its slot
+    c.extend([a], [100])
+    assert c.extend([a], [150]) == [250] and c.room(a) == 6
+
+
+def test_forks_of_short_rings_know_what_is_gone():
+    from yalm_amd.cache import CacheFull
+    c = _windows(256, 8192, (100,), max_draft=70)
+    assert c.kv_groups[0].ring_pages == 4
+    c = _windows(128, 8192, (100,), max_draft=70)
+    (a,) = c.acquire(1)
+    c.extend([a], [10])
+    (b,), _ = c.fork(a, 1)
+    assert c.room(b) == c.room(a) == 118
+    c.release([a, b])
+    (a,) = c.acquire(1)
+    c.extend([a], [129])                               # pages 1 and 2 are held, position 129 sees from 30 on
+    with pytest.raises(CacheFull, match="window"):
+        c.extend([a], [1])

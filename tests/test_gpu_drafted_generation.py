@@ -318,3 +318,42 @@ def test_draws_behind_refused_ones():
             if len(waiting) == Sampler.HOST_BUFFERS:
                 got.append(waiting.pop(0).tolist())
         assert got + [d.tolist() for d in waiting] == want
+
+
+@pytest.mark.parametrize("window,max_tokens,max_nodes", [(64, 512, 16), (64, 64, 16), (63, 128, 20), (40, 64, 9), (200, 128, 5)])
+def test_drafted_generation_to_the_end_where_a_window_is_as_long_as_the_context(folders, window, max_tokens, max_nodes):
+    """Trees near the end of the context lie behind it, or are cut where the pages end: the tokens are generate()'s, by guesses that are
+    right, by ones that are wrong and by the text's own."""
+    from yalm_amd import Engine, Model, generate, generate_drafted
+    engine = Engine(Model.from_folder(folders["tiny_mistral"], dtype=torch.float32, device="cuda:0", window=window), max_tokens=max_tokens, max_batch=2, max_draft=20)
+    limit = engine.n_positions
+    assert limit == tiny_configs.ALL["tiny_mistral"]["max_position_embeddings"]
+    prompt = [5, 9, 31] * 4
+    want = generate(engine, [prompt], max_new_tokens=limit, stop_ids=[])
+    assert len(prompt) + len(want[0]) == limit
+
+    def oracle(history, n):
+        ahead = (prompt + want[0])[len(history) - 1:][:n - 1] + [7]
+        return ahead + [8] * (n - len(ahead)), list(range(-1, len(ahead) - 1)) + [0] * (n - len(ahead))
+
+    wrong = lambda history, n: ([history[-1]] + [0] * (n - 1), [-1] + [0] * (n - 1))  # noqa: E731
+    for guess in ({}, {"guess": oracle}, {"guess": wrong}):
+        assert generate_drafted(engine, [prompt], max_new_tokens=limit, stop_ids=[], max_nodes=max_nodes, **guess) == want
+    assert not engine.cache.slots.held and all(g.pool.n_free == g.n_pages for g in engine.cache.kv_groups)
+
+
+def test_what_outgrows_a_window_s_pages_is_refused(folders):
+    """Drafted tokens that would lie on keys in sight, and a plain step that would: nothing changes, and what fits goes on."""
+    from yalm_amd import Engine, Model, StepError
+    engine = Engine(Model.from_folder(folders["tiny_mistral"], dtype=torch.float32, device="cuda:0", window=100), max_tokens=64, max_batch=1, max_draft=20, positions=200)
+    (s,) = engine.start(1)
+    engine.step([s], [list(range(3, 60))])
+    with pytest.raises(StepError, match="window"):
+        engine.draft_step([s], [[1] * 8])
+    engine.draft_step([s], [[1] * 7])
+    engine.keep([s], [[0, 1, 2, 3, 4, 5, 6]])
+    assert engine.length(s) == 64
+    for call in (lambda: engine.step([s], [[1]]), lambda: engine.draft_step([s], [[1]])):
+        with pytest.raises(StepError, match="window"):
+            call()
+    engine.release([s])

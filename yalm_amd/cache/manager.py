@@ -146,11 +146,15 @@ class KVGroup:
         self.dtype = dtype
         self.window = request.window
         full_pages = max(1, pages_for(max_seq_len))
+        self.ring_pages, self.short = full_pages, False
         if self.window > 0:
             # drafted tokens lie behind the ones that the first of them sees
-            self.ring_pages = min(full_pages, pages_for(self.window + max(max_draft - 1, 0)) + 1)
-        else:
-            self.ring_pages = full_pages
+            whole = pages_for(self.window + max(max_draft - 1, 0)) + 1
+            self.ring_pages = min(full_pages, whole)
+            # A short ring comes round to keys that a window still sees if a sequence outgrows it.  Then what it still holds of each slot's
+            # sequence is known by its first position, and who would go on without a key in sight is refused.
+            self.short = whole > full_pages
+        self.first_held = [0] * n_slots
         self.n_pages = n_pages
         self.pool = PagePool(n_pages)
         H, hd = request.n_kv_heads, request.head_dim
@@ -191,6 +195,17 @@ class KVGroup:
         have = min(pages_for(old_len), self.ring_pages)
         need = min(pages_for(new_len), self.ring_pages)
         return max(0, need - have)
+
+    def room(self, slot, length):
+        """The most tokens that a sequence of `length` can go on by at once so that the ring holds every key that the first of them sees."""
+        sees = max(0, length - self.window + 1)
+        return sees + self.ring_pages * PAGE - length if self.first_held[slot] <= sees else 0
+
+    def note(self, slot, old_len, new_len):
+        """What is left of a sequence in a short ring when it has grown: of a whole prompt its last pages, of tokens behind it all that no
+        later one lies on."""
+        gone = new_len - self.ring_pages * PAGE if old_len > 0 else (pages_for(new_len) - self.ring_pages) * PAGE
+        self.first_held[slot] = max(self.first_held[slot], gone)
 
     def grow(self, slots, old_lens, new_lens):
         """Takes the pages that the sequences in `slots` need to grow from old_lens to new_lens.
@@ -233,6 +248,7 @@ class KVGroup:
                     copies.append((page, to))
                     page = to
                 self.table_host[s, col] = page
+            self.first_held[s] = self.first_held[slot]
             self._dirty.add(s)
         return copies
 
@@ -256,6 +272,7 @@ class KVGroup:
             if row[col] >= 0:
                 self.pool.give_back(int(row[col]))
                 row[col] = -1
+        self.first_held[slot] = 0
         self._dirty.add(slot)
 
     def flush(self):
@@ -306,9 +323,10 @@ class CacheManager:
     layer made of several members that keep something has the line (id, name) for each}
     max_tokens: the most tokens live sequences hold at any time, each sequence's
     count rounded up to a multiple of PAGE.  max_draft: the most drafted tokens that a sequence goes on by at once (the rings
-    of windowed groups have room for them)."""
+    of windowed groups have room for them).  longest: how long a sequence may grow where every group keeps a window (default: max_seq_len;
+    a text may run past the model's positions then)."""
 
-    def __init__(self, requests, max_tokens, max_seq_len, dtype, device, n_slots=None, max_draft=0):
+    def __init__(self, requests, max_tokens, max_seq_len, dtype, device, n_slots=None, max_draft=0, longest=None):
         if max_tokens <= 0:
             raise CacheError("max_tokens must be positive")
         self.device = device
@@ -331,9 +349,13 @@ class CacheManager:
         self.kv_groups = []
         self.state_groups = []
         self._group_of_line = {}
+        self.unbounded = all(r.window > 0 for r in by_request if isinstance(r, KVRequest))     # no group keeps every key
+        group_len = self.max_seq_len
+        if self.unbounded:                             # drafts of the last tokens lie behind the longest sequence's end
+            group_len = min(max(max_seq_len, longest or 0) + max(max_draft - 1, 0), self.n_pages * PAGE)
         for req, lines in by_request.items():
             if isinstance(req, KVRequest):
-                g = KVGroup(req, sorted(lines, key=_line_order), self.n_pages, self.n_slots, self.max_seq_len, dtype, device, max_draft)
+                g = KVGroup(req, sorted(lines, key=_line_order), self.n_pages, self.n_slots, group_len, dtype, device, max_draft)
                 self.kv_groups.append(g)
             elif isinstance(req, StateRequest):
                 g = StateGroup(req, sorted(lines, key=_line_order), self.n_slots, device)
@@ -342,7 +364,7 @@ class CacheManager:
                 raise CacheError("unknown cache request %r" % (req,))
             for l in lines:
                 self._group_of_line[l] = g
-        self.unbounded = all(g.window > 0 for g in self.kv_groups)     # no group keeps every key
+        self._short = [g for g in self.kv_groups if g.short] if self.unbounded else []       # else no sequence outgrows a ring
 
     def group_of(self, line):
         return self._group_of_line.get(line)
@@ -378,6 +400,11 @@ class CacheManager:
         if not self.unbounded and max(new_lens) > self.max_seq_len:
             raise CacheFull("a sequence of %d tokens exceeds the longest the cache holds (%d)"
                             % (max(new_lens), self.max_seq_len))
+        for g in self._short:
+            for s, o, n in zip(slots, old_lens, n_new):
+                if o > 0 and n > g.room(s, o):
+                    raise CacheFull("a sequence of %d tokens cannot go on by %d: the cache's %d pages do not hold all that a window of %d positions "
+                                    "sees (max_tokens too small)" % (o, n, g.ring_pages, g.window))
         # only a sequence that passes a page's end can need a page, in whatever group
         growing = [i for i, (o, n) in enumerate(zip(old_lens, new_lens)) if (o + PAGE - 1) // PAGE != (n + PAGE - 1) // PAGE]
         if growing:
@@ -393,9 +420,19 @@ class CacheManager:
                 g.grow(g_slots, g_old, g_new)
         for g in self.kv_groups:
             g.flush()
+        for g in self._short:
+            for s, o, n in zip(slots, old_lens, new_lens):
+                g.note(s, o, n)
         for s, nl in zip(slots, new_lens):
             seq_len[s] = nl
         return new_lens
+
+    def room(self, slot):
+        """The most tokens that a sequence can go on by at once, however many pages are free."""
+        n = self.seq_len[slot]
+        if not self.unbounded:
+            return self.max_seq_len - n
+        return min([g.room(slot, n) for g in self._short], default=1 << 30)
 
     def fork(self, slot, n):
         """n fresh slots that hold what `slot` holds (its tokens so far), and the copies that make it so: [(tensor, its companion or None,

@@ -105,8 +105,7 @@ def generate_drafted(engine, prompts, max_new_tokens=256, temperature=0.0, seed=
                     history = list(prompts[i]) + results[i]
                     # no deeper than the request's tokens, the context and a window go, and no wider than the places behind its tokens
                     left = min(max_new_tokens - len(results[i]), max_len - len(history), engine.max_draft_depth)
-                    tokens, parents = guess(history, max(1, min(max_nodes, engine.cache.max_seq_len - engine.length(s) if not engine.cache.unbounded
-                                                                else max_nodes)))
+                    tokens, parents = guess(history, max(1, min(max_nodes, max_len - engine.length(s), engine.cache.room(s))))
                     trees.append(_shallow(tokens, parents, left))
                 running = [s for _, s in live]
                 logits = engine.draft_step(running, [t for t, _, _ in trees], [p for _, p, _ in trees])

@@ -97,7 +97,8 @@ class Engine:
         self.device = model.device
         self.dtype = model.compute_dtype
         self.cache = CacheManager(model.cache_requests(), max_tokens, model.spec.max_positions, self.dtype,
-                                  self.device, n_slots=max_batch, max_draft=min(int(max_draft), kernels.MAX_TREE_NODES) if model.takes_drafts() else 0)
+                                  self.device, n_slots=max_batch, max_draft=min(int(max_draft), kernels.MAX_TREE_NODES) if model.takes_drafts() else 0,
+                                  longest=None if positions is None else int(positions))
         windowed = any(g.window > 0 for g in self.cache.kv_groups)
         self.max_draft = min(int(max_draft), kernels.MAX_TREE_NODES) if windowed else kernels.MAX_TREE_NODES
         # a node sees its root: depths stay below the narrowest window
