@@ -331,3 +331,58 @@ def test_forks_of_short_rings_know_what_is_gone():
     c.extend([a], [129])                               # pages 1 and 2 are held, position 129 sees from 30 on
     with pytest.raises(CacheFull, match="window"):
         c.extend([a], [1])
+
+
+def test_cuts_that_would_write_on_for_others_are_refused():
+    """A page that a fork shares is whole for everyone who holds it: who were cut into one would write on in it."""
+    from yalm_amd.cache import CacheError
+    c = _windows(1024, 1024, (0, 100))
+    a, z = c.acquire(2)
+    c.extend([a, z], [150, 10])
+    (b,), _ = c.fork(a, 1)
+    g = c.kv_groups[0] if c.kv_groups[0].window == 0 else c.kv_groups[1]
+
+    def state():
+        return list(c.seq_len), [(h.pool.n_free, h.table_host.tolist()) for h in c.kv_groups]
+
+    before = state()
+    for slots, lengths in (([a], [127]), ([b], [100]), ([b], [1]), ([z, a], [5, 70]), ([a, a], [149, 150]), ([a, a], [150, 149]), ([a, z], [150]), ([z], [11])):
+        with pytest.raises(CacheError):
+            c.cut(slots, lengths)
+        assert state() == before
+    c.cut([a, b], [130, 128])                          # behind what they share
+    assert g.pool.holders(int(g.table_host[a, 0])) == 2 and (g.table_host[b, 2:] == -1).all()
+    c.extend([b], [3])
+    assert int(g.table_host[b, 2]) != int(g.table_host[a, 2])
+    c.cut([b], [64])                                   # a page's end: the next token starts a page of its own
+    c.extend([b], [1])
+    assert int(g.table_host[b, 0]) == int(g.table_host[a, 0]) and g.pool.holders(int(g.table_host[b, 1])) == 1 and g.table_host[b, 1] != g.table_host[a, 1]
+    c.release([b])
+    c.cut([a], [100])                                  # nobody else holds it any more
+    c.release([a, z])
+    assert all(h.pool.n_free == h.n_pages for h in c.kv_groups)
+
+
+@pytest.mark.parametrize("max_tokens", [1024, 128])
+def test_cuts_to_where_a_window_s_keys_are_gone_are_refused(max_tokens):
+    from yalm_amd.cache import CacheError
+    c = _windows(max_tokens, 8192, (100,), max_draft=20)
+    lines = Lines(c)
+    (a,) = c.acquire(1)
+    lines.grow(a, 90)
+    for _ in range(300):
+        lines.grow(a, 1)
+    ring = c.kv_groups[0].ring_pages * 64
+    assert ring == (192 if max_tokens == 1024 else 128)
+    first, more = 390 - ring + 99, 63 if max_tokens == 1024 else 20      # from `first` on the next token sees what is held; pages count whole
+    with pytest.raises(CacheError, match="window"):
+        c.cut([a], [first - 64])
+    assert c.seq_len[a] == 390
+    c.cut([a], [first + more])
+    lines.check(a, *lines.grow(a, 1))
+    c.cut([a], [first + more])
+    with pytest.raises(CacheError, match="window"):    # what was written behind does not come back by steps
+        for n in range(first + more - 1, first - 65, -1):
+            c.cut([a], [n])
+            old, new = lines.grow(a, 1)
+            lines.check(a, old, new)

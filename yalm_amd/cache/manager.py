@@ -151,9 +151,9 @@ class KVGroup:
             # drafted tokens lie behind the ones that the first of them sees
             whole = pages_for(self.window + max(max_draft - 1, 0)) + 1
             self.ring_pages = min(full_pages, whole)
-            # A short ring comes round to keys that a window still sees if a sequence outgrows it.  Then what it still holds of each slot's
-            # sequence is known by its first position, and who would go on without a key in sight is refused.
+            # A short ring comes round to keys that a window still sees if a sequence outgrows it: who would go on without one is refused.
             self.short = whole > full_pages
+        # the first position of each slot's sequence that a ring still holds: kept for short rings as they grow, for whole ones only behind cuts
         self.first_held = [0] * n_slots
         self.n_pages = n_pages
         self.pool = PagePool(n_pages)
@@ -256,8 +256,26 @@ class KVGroup:
         """The pages that fork_pages takes for n slots."""
         return n * (self.columns(length) - (0 if self.window > 0 else length // PAGE))
 
+    def check_cut(self, slot, old_len, new_len):
+        """Refuses a cut behind which the sequence would write on in a page that others hold, or go on without a key in its window's sight."""
+        if new_len == old_len:
+            return
+        if self.window > 0:
+            if self._gone(slot, old_len) > max(0, new_len - self.window + 1):
+                raise CacheError("slot %r of %d tokens cannot be cut to %d: the ring no longer holds all that a window of %d positions sees from there"
+                                 % (slot, old_len, new_len, self.window))
+        elif new_len % PAGE and self.pool.holders(int(self.table_host[slot, new_len // PAGE])) > 1:
+            raise CacheError("slot %r of %d tokens cannot be cut to %d: other sequences hold the page that it would write on in" % (slot, old_len, new_len))
+
+    def _gone(self, slot, length):
+        """How many of a sequence's first positions a ring may hold no more."""
+        gone = self.first_held[slot]
+        return gone if self.short else max(gone, (pages_for(length) - self.ring_pages) * PAGE)
+
     def cut(self, slot, old_len, new_len):
         """Gives back the pages behind new_len of a sequence of old_len tokens (those of a ring stay: it keeps them all)."""
+        if self.window > 0:
+            self.first_held[slot] = self._gone(slot, old_len)
         if self.window > 0 and pages_for(new_len) >= self.ring_pages:
             return
         row = self.table_host[slot]
@@ -466,10 +484,15 @@ class CacheManager:
         return new, copies
 
     def cut(self, slots, lengths):
-        """Shortens sequences to the given lengths; the pages behind them are given back."""
+        """Shortens sequences to the given lengths; the pages behind them are given back.  Nothing changes if one of them cannot go on from there:
+        its last page is shared, or its window sees keys that the ring has come round to."""
+        if len(lengths) != len(slots) or len(set(slots)) != len(slots):
+            raise CacheError("a cut needs one length for each of its slots, and each slot once")
         for s, n in zip(slots, lengths):
             if not self.slots.is_held(s) or not 0 <= n <= self.seq_len[s]:
                 raise CacheError("slot %r of %d tokens cannot be cut to %r" % (s, self.seq_len[s], n))
+            for g in self.kv_groups:
+                g.check_cut(s, self.seq_len[s], n)
         for s, n in zip(slots, lengths):
             for g in self.kv_groups:
                 g.cut(s, self.seq_len[s], n)
