@@ -381,7 +381,7 @@ __device__ __forceinline__ void tree_leave(const TreeArgs& a, const TreeSeq& s, 
       for (int r = 0; r < 4; ++r) r4[r] = from_f32<T>(o[dt][r] * inv);
       *reinterpret_cast<out4*>(rows + j * ROW + dt * 16 + 4 * qd) = r4;
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_order();
 #pragma unroll
     for (int i = lane; i < 16 * PIECES; i += WAVE)
       if (const int x = x0 + i / PIECES; x < cols)
@@ -397,7 +397,7 @@ __device__ __forceinline__ void tree_leave(const TreeArgs& a, const TreeSeq& s, 
       if (qd == 0) *reinterpret_cast<float2*>(to + HD) = make_float2(m, l);
     }
   }
-  __builtin_amdgcn_wave_barrier();                 // the next tile takes the same place
+  wave_order();                                    // the next tile takes the same place
 }
 
 // ---------------------------------------------------------------------------

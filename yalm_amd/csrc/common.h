@@ -147,6 +147,16 @@ __device__ __forceinline__ float wave_max(float v) {
   return wave_fold(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
+// Between what some lanes of a wave leave in LDS and what others of the same wave read there, either way round.  A wave's accesses to
+// LDS happen in the order in which it issues them, so this is no instruction: it keeps the compiler from another order.
+__device__ __forceinline__ void wave_order() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#endif
+}
+
 // Sum over a block of NW waves; every thread gets the result.  `red` holds NW floats.
 template <int NW>
 __device__ __forceinline__ float block_sum(float v, float* red) {

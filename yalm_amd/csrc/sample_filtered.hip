@@ -1076,10 +1076,12 @@ __device__ __forceinline__ void last_of_few(const Step& st, int row, const Wish&
   const int lane = threadIdx.x;
   u64* y = x + WAVE;
   x[lane] = lane < n ? order : ~0ull;
+  wave_order();
   int rank = 0;
 #pragma unroll 8
   for (int j = 0; j < (n + 7) / 8 * 8; ++j) rank += x[j] < order;
   if (lane < n) y[rank] = order;
+  wave_order();
   order = y[lane];                               // the token of this rank (lanes from n on: anything)
   const float l = logit_of(order);
   set_scale(r, logit_of(first_lane(order)), want.T);
@@ -1090,10 +1092,12 @@ __device__ __forceinline__ void last_of_few(const Step& st, int row, const Wish&
   const int kept = __popcll(__ballot(in));       // the first ones
   const unsigned index = in ? (unsigned)order : 0xFFFFFFFFu;
   x[lane] = index;
+  wave_order();
   int place = 0;
 #pragma unroll 8
   for (int j = 0; j < (kept + 7) / 8 * 8; ++j) place += (unsigned)x[j] < index;
   if (in) y[place] = order;
+  wave_order();
   const u64 mine = y[lane];
   const float ml = logit_of(mine);
   const u64 mw = lane < kept ? r.weight(ml) : 0, reach = wave_scan(mw), sum = last_lane(reach), target = want.target(sum);
