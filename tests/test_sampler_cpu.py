@@ -1,4 +1,5 @@
 """The sampler's buffers without a GPU: stand-ins for its kernels write each draw's own number, pinned memory and events are plain ones."""
+import numpy as np
 import pytest
 import torch
 
@@ -88,3 +89,27 @@ def test_draws_under_filters_have_workspaces_of_their_own(stand_in):
     draws = [s.draw(torch.zeros((2, 5)), 0.7, [0, 1], [i, i], top_p=0.9) for i in range(3)]
     assert len({w.data_ptr() for w in stand_in["workspaces"]}) == 3 and all(w.numel() >= 12 for w in stand_in["workspaces"])
     assert [d.tolist() for d in draws] == [[i, i] for i in range(3)]
+
+
+class NoEngine:
+    """An engine that a refused call never touches."""
+    n_positions, max_draft, max_draft_depth = 64, 8, 8
+
+    def __getattr__(self, name):
+        raise AssertionError("the engine's %s was asked for" % name)
+
+
+@pytest.mark.parametrize("loop", ["generate", "generate_drafted"])
+@pytest.mark.parametrize("name,value", [("top_k", [3, 5]), ("top_k", np.array([3, 5])), ("top_p", torch.tensor([0.5, 0.9])), ("min_p", (0.1, 0.1)), ("temperature", [0.7, 0.8]),
+                                        ("temperature", np.full(2, 0.5)), ("top_k", -1), ("top_p", 1.5), ("min_p", float("nan"))])
+def test_loops_take_one_number_for_all_requests(loop, name, value):
+    """Refused before the first step, where a sequence failed once the first request had left its batch, and the others' tokens with it."""
+    import yalm_amd
+    with pytest.raises(ValueError, match=name):
+        getattr(yalm_amd, loop)(NoEngine(), [[1, 2], [3]], stop_ids=[], max_new_tokens=4, sampler=Sampler(1), **{name: value})
+
+
+def test_a_loop_s_numbers_of_any_kind():
+    from yalm_amd.sampling.sampler import filters_for_all
+    assert filters_for_all(0, 1.0, 0.0) == filters_for_all(np.int64(0), np.float32(1), torch.tensor(0.0)) == filters_for_all(0, 1, 0) == {}
+    assert filters_for_all(np.array(7), torch.tensor(0.5), 0) == {"top_k": 7, "top_p": 0.5, "min_p": 0.0}

@@ -53,14 +53,17 @@ def generate_drafted(engine, prompts, max_new_tokens=256, temperature=0.0, seed=
     """As generate() (without `ahead`: a step's tree hangs on the tokens of the step before).  guess(history, n): the (tokens, parents) of a tree
     of at most n nodes behind a request's prompt and new tokens, the root being the last of them."""
     from .sampling import Sampler
+    from .sampling.sampler import filters_for_all, one_for_all
     sampler = sampler or Sampler(seed)
+    filters = filters_for_all(top_k, top_p, min_p)
+    if isinstance(sampler, Sampler):
+        one_for_all("temperature", temperature)
     stats = stats if stats is not None else GenerationStats()
     stop = set(stop_ids if stop_ids is not None else getattr(engine.model.spec, "eos_token_ids", None) or [])
     ids = list(request_ids) if request_ids is not None else list(range(len(prompts)))
     max_len, max_nodes = engine.n_positions, int(max_nodes)
     if not 1 <= max_nodes <= engine.max_draft:
         raise ValueError("trees of %d nodes: the engine takes 1 to %d" % (max_nodes, engine.max_draft))
-    filters = {} if (top_k, top_p, min_p) == (0, 1.0, 0.0) else {"top_k": top_k, "top_p": top_p, "min_p": min_p}
     results = [[] for _ in prompts]
     if max_new_tokens <= 0 or not prompts:
         return results

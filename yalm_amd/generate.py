@@ -72,7 +72,8 @@ def plan_batches(prompt_lens, max_new_tokens, batch_size, max_tokens, n_slots, m
 def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_ids=None, batch_size=None,
              sampler=None, on_token=None, stats=None, request_ids=None, ahead=None, top_k=0, top_p=1.0, min_p=0.0, samples=1):
     """Generates for every prompt (a list of token ids).  Returns the new tokens of
-    each request, in the order of the prompts.  top_k, top_p, min_p: see Sampler.draw.  samples > 1: every prompt is answered that many
+    each request, in the order of the prompts.  top_k, top_p, min_p: see Sampler.draw, here one number
+    for all requests, as the temperature is.  samples > 1: every prompt is answered that many
     times and runs once (its sequence is forked behind the prompt step); the answers of prompt i are the requests samples * i, samples * i + 1,
     ... of the result and of on_token, drawn as requests of the ids samples * id, samples * id + 1, ...  stop_ids None means the model's own
     (config eos); on_token(request index, token) is called for every new token.
@@ -86,7 +87,11 @@ def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_
     matter: its products take the tiles that its number of tokens asks for, which add in different orders, so that a request's
     prompt logits move in their last bits with the prompts that start beside it, in float32 too."""
     from .sampling import Sampler
+    from .sampling.sampler import filters_for_all, one_for_all
     sampler = sampler or Sampler(seed)
+    filters = filters_for_all(top_k, top_p, min_p)
+    if isinstance(sampler, Sampler):
+        one_for_all("temperature", temperature)
     stats = stats if stats is not None else GenerationStats()
     if stop_ids is None:
         stop_ids = list(getattr(engine.model.spec, "eos_token_ids", []) or [])
@@ -105,7 +110,6 @@ def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_
     if samples > 1:
         prompts = [p for p in prompts for _ in range(samples)]
         ids = [samples * r + k for r in ids for k in range(samples)]
-    filters = {} if (top_k, top_p, min_p) == (0, 1.0, 0.0) else {"top_k": top_k, "top_p": top_p, "min_p": min_p}
     results = [[] for _ in prompts]
     if max_new_tokens <= 0 or not prompts:
         return results

@@ -156,3 +156,17 @@ class Sampler:
         out = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
         kernels.token_prob(logits, idx, out)
         return out.tolist()
+
+
+def filters_for_all(top_k, top_p, min_p):
+    """What a loop whose batches shrink hands to every draw: one number for all requests each, checked before the first step ({}: all are off)."""
+    settings = {"top_k": top_k, "top_p": top_p, "min_p": min_p}
+    for name, value in settings.items():
+        one_for_all(name, value)
+    settings = Sampler._checked(settings, 0)
+    return {} if tuple(settings.values()) == (0, 1.0, 0.0) else settings
+
+
+def one_for_all(name, value):
+    if _of_rows(value):
+        raise ValueError("%s: a generation loop takes one number for all requests (Sampler.draw takes one for each row)" % name)
