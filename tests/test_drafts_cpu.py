@@ -386,3 +386,74 @@ def test_cuts_to_where_a_window_s_keys_are_gone_are_refused(max_tokens):
             c.cut([a], [n])
             old, new = lines.grow(a, 1)
             lines.check(a, old, new)
+
+
+# ------------------------------------------------------------------------------------------------ the drafting loop without a GPU
+class ScriptedDrafts:
+    """An engine whose model says at each place of request r the token 7 r + place: nothing but the loop's decisions is run."""
+    max_draft, max_draft_depth = 256, 256
+
+    class _Cache:
+        unbounded, max_seq_len = False, 4096
+
+        def __init__(self, n_slots, n_pages):
+            self.n_slots, self.n_pages = n_slots, n_pages
+
+        def room(self, slot):
+            return 1 << 30
+
+    def __init__(self, n_slots=8, n_pages=400, n_positions=4096, most=None):
+        self.cache, self.n_positions = self._Cache(n_slots, n_pages), n_positions
+        self.lens, self.sizes, self.free, self.pending = {}, [], list(range(n_slots)), {}
+        if most is not None:
+            self.max_step_drafts = most
+
+    def start(self, n):
+        out = [self.free.pop(0) for _ in range(n)]
+        self.lens.update({s: 0 for s in out})
+        return out
+
+    def release(self, slots):
+        for s in slots:
+            del self.lens[s]
+            self.free.append(s)
+
+    def length(self, slot):
+        return self.lens[slot]
+
+    def step_bytes(self, slots):
+        return 0
+
+    def step(self, slots, tokens):
+        for s, t in zip(slots, tokens):
+            self.lens[s] += len(t)
+        return None
+
+    def draft_step(self, slots, tokens, parents):
+        assert all(len(p) == len(t) for p, t in zip(parents, tokens))
+        self.sizes.append([len(t) for t in tokens])
+        assert sum(self.sizes[-1]) <= getattr(self, "max_step_drafts", 1 << 30)
+        return None
+
+    def keep(self, slots, paths):
+        for s, path in zip(slots, paths):
+            self.lens[s] += len(path)
+
+
+class ScriptedTokens:
+    def sample(self, logits, temperature, request_ids, steps):
+        return [7 * r + s for r, s in zip(request_ids, steps)]
+
+
+def chain_guess(history, n):
+    return [history[-1] + k for k in range(n)], list(range(-1, n - 1))
+
+
+@pytest.mark.parametrize("most", [None, 1000, 100, 17, 8])
+def test_a_step_s_drafts_stay_within_the_engine_s_limit(most):
+    """Trees of a full batch are cut to what one step takes, in place of a refusal behind the prompts, with all results lost."""
+    from yalm_amd import generate_drafted
+    engine = ScriptedDrafts(most=1 << 30 if most is None else most)
+    out = generate_drafted(engine, [[5] * (i + 1) for i in range(8)], max_new_tokens=300, stop_ids=[], sampler=ScriptedTokens(), guess=chain_guess, max_nodes=64)
+    assert out == [[7 * r + s for s in range(300)] for r in range(8)]
+    assert max(max(x) for x in engine.sizes) == min(64, (most or 1 << 30) // 8 if most != 17 else 2) and not engine.lens

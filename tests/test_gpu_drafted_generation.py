@@ -357,3 +357,23 @@ def test_what_outgrows_a_window_s_pages_is_refused(folders):
         with pytest.raises(StepError, match="window"):
             call()
     engine.release([s])
+
+
+def test_drafts_of_a_full_batch_stay_within_a_step_s_limit(folders):
+    """An engine whose steps take few elements: trees are cut to a share of them, where a step was refused behind the prompts."""
+    from yalm_amd import StepError, generate, generate_drafted
+    engine = engine_of(folders, "tiny_mistral", torch.float32)
+    widest = max(engine._widest_row, engine.model.vocab_size)
+    prompts = [[7, 3, 9, 7, 3], [5, 6, 5, 6], [11] * 6, [2, 4, 8, 2, 4]]
+    want = generate(engine, prompts, max_new_tokens=20, stop_ids=[])
+    wide = lambda history, n: ([history[-1]] + [0] * (n - 1), [-1] + [0] * (n - 1))  # noqa: E731
+    engine.MAX_ELEMENTS = 24 * widest + 1
+    assert engine.max_step_drafts == 24
+    assert generate_drafted(engine, prompts, max_new_tokens=20, stop_ids=[], max_nodes=20, guess=wide) == want
+    assert generate_drafted(engine, prompts, max_new_tokens=20, stop_ids=[], max_nodes=20) == want
+    slots = engine.start(2)
+    engine.step(slots, [[1], [2]])
+    with pytest.raises(StepError, match="25 drafted"):
+        engine.draft_step(slots, [[1] * 20, [1] * 5])
+    engine.draft_step(slots, [[1] * 20, [1] * 4])
+    engine.release(slots)

@@ -104,11 +104,12 @@ def generate_drafted(engine, prompts, max_new_tokens=256, temperature=0.0, seed=
                 if not live:
                     break
                 trees = []
+                share = min(max_nodes, engine.max_step_drafts // len(live))       # of what one step takes
                 for i, s in live:
                     history = list(prompts[i]) + results[i]
                     # no deeper than the request's tokens, the context and a window go, and no wider than the places behind its tokens
                     left = min(max_new_tokens - len(results[i]), max_len - len(history), engine.max_draft_depth)
-                    tokens, parents = guess(history, max(1, min(max_nodes, max_len - engine.length(s), engine.cache.room(s))))
+                    tokens, parents = guess(history, max(1, min(share, max_len - engine.length(s), engine.cache.room(s))))
                     trees.append(_shallow(tokens, parents, left))
                 running = [s for _, s in live]
                 logits = engine.draft_step(running, [t for t, _, _ in trees], [p for _, p, _ in trees])

@@ -301,7 +301,7 @@ class Engine:
             raise StepError("token id %r is outside the vocabulary of %d" % (bad[0], V))
         words = (max(n_tok) + 63) // 64
         T = sum(n_tok)
-        if T * max(self._widest_row, V) >= self.MAX_ELEMENTS:
+        if T > self.max_step_drafts:
             raise StepError("a step of %d drafted tokens is refused: its widest buffer (%d elements a token) would reach 2^31 elements"
                             % (T, max(self._widest_row, V)))
         trees, depths, masks = [], [], np.zeros((T, words), dtype=np.uint64)
@@ -344,6 +344,11 @@ class Engine:
         logits = self.ws.get("logits", (T, V), torch.float32)
         self.model.forward(ctx, None, logits)
         return logits
+
+    @property
+    def max_step_drafts(self):
+        """The most drafted tokens, of all sequences together, that one draft_step takes."""
+        return (self.MAX_ELEMENTS - 1) // max(self._widest_row, self.model.vocab_size)
 
     def keep(self, slots, paths):
         """Ends a draft_step of these sequences: paths[i] are the drafted tokens of slots[i] that it goes on with, a path from the tree's root
