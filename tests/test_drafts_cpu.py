@@ -402,6 +402,9 @@ class ScriptedDrafts:
         def room(self, slot):
             return 1 << 30
 
+        def whole_rings(self):
+            return 0
+
     def __init__(self, n_slots=8, n_pages=400, n_positions=4096, most=None):
         self.cache, self.n_positions = self._Cache(n_slots, n_pages), n_positions
         self.lens, self.sizes, self.free, self.pending = {}, [], list(range(n_slots)), {}

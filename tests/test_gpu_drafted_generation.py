@@ -374,6 +374,33 @@ def test_drafts_of_a_full_batch_stay_within_a_step_s_limit(folders):
     slots = engine.start(2)
     engine.step(slots, [[1], [2]])
     with pytest.raises(StepError, match="25 drafted"):
-        engine.draft_step(slots, [[1] * 20, [1] * 5])
-    engine.draft_step(slots, [[1] * 20, [1] * 4])
+        engine.draft_step(slots, [[1] * 20, [1] * 5], [[-1] + [0] * 19, [-1] + [0] * 4])
+    engine.draft_step(slots, [[1] * 20, [1] * 4], [[-1] + [0] * 19, [-1] + [0] * 3])
     engine.release(slots)
+
+
+@pytest.mark.parametrize("how", [{"context": 24}, {"window": 22}])
+def test_texts_that_run_past_the_cache_s_tokens(folders, how):
+    """A window's ring holds a text however long it runs: a few pages serve for hundreds of tokens, with drafts and without."""
+    from yalm_amd import Engine, Model, generate, generate_drafted
+    model = Model.from_folder(folders["tiny_mistral"], dtype=torch.float32, device="cuda:0", **how)
+    prompts, n_new = [[1, 17, 200, 33, 5], [5, 9] * 40], 300
+    at = dict(positions=400, max_batch=2, max_draft=9)
+    args = dict(max_new_tokens=n_new, stop_ids=[])
+    want = generate(Engine(model, max_tokens=1024, **at), prompts, **args)
+    assert [len(w) for w in want] == [n_new] * 2
+    small = Engine(model, max_tokens=256, **at)
+    assert generate(small, prompts, **args) == want
+    if "window" in how:
+        assert generate_drafted(small, prompts, max_nodes=9, **args) == want
+    assert all(g.pool.n_free == g.n_pages for g in small.cache.kv_groups)
+
+
+def test_the_command_line_runs_a_text_past_its_context(folders, capsys):
+    from yalm_amd import Engine, Model, generate
+    from yalm_amd.cli import main
+    model = Model.from_folder(folders["tiny_mistral"], dtype=torch.float32, device="cuda:0", context=24)
+    want = generate(Engine(model, max_tokens=1024, positions=700), [[1, 17, 200]], max_new_tokens=500, stop_ids=[])[0]
+    main([folders["tiny_mistral"], "--tokens", "1,17,200", "-n", "500", "-t", "0", "-T", "24", "--dtype", "float32"])
+    stop = tiny_configs.ALL["tiny_mistral"].get("eos_token_id")
+    assert " ".join(map(str, want[:want.index(stop) + 1] if stop in want else want)) in capsys.readouterr().out

@@ -452,6 +452,12 @@ class CacheManager:
             return self.max_seq_len - n
         return min([g.room(slot, n) for g in self._short], default=1 << 30)
 
+    def whole_rings(self):
+        """The most pages of a group that a sequence holds however long it grows; 0: it holds more as it grows, or cannot grow beyond them."""
+        if not self.unbounded or self._short:
+            return 0
+        return max([g.ring_pages for g in self.kv_groups], default=0)
+
     def fork(self, slot, n):
         """n fresh slots that hold what `slot` holds (its tokens so far), and the copies that make it so: [(tensor, its companion or None,
         [from], [to])], blocks numbered along the second dimension of each tensor.  The copies are to be queued before anything else touches

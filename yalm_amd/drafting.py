@@ -4,6 +4,7 @@ it would have drawn behind each of them, and the path of guesses that it agrees 
 The tokens are those of generate() with the same seed, up to rounding: the token of a place is drawn from the model's own logits there, with
 the number that belongs to the request and the place, and a guess is kept only if it is that token.  A guesser that is never right
 costs a step of wider rows a token; each guess that is right saves a step."""
+from .cache.manager import PAGE
 from .generate import GenerationStats, plan_batches
 
 
@@ -82,7 +83,8 @@ def generate_drafted(engine, prompts, max_new_tokens=256, temperature=0.0, seed=
 
     import time
     room = max_new_tokens + max_nodes                 # drafted tokens lie in the cache beside the kept ones
-    for batch in plan_batches([len(p) for p in prompts], room, batch_size, engine.cache.n_pages * 64, engine.cache.n_slots, max_len):
+    for batch in plan_batches([len(p) for p in prompts], room, batch_size, engine.cache.n_pages * PAGE, engine.cache.n_slots, max_len,
+                              engine.cache.whole_rings()):
         stats.batches += 1
         stats.batch_sizes.append(len(batch))
         slots = engine.start(len(batch))

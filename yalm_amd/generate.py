@@ -43,10 +43,11 @@ class GenerationStats:
         return n / self.decode_seconds if self.decode_seconds > 0 else 0.0
 
 
-def plan_batches(prompt_lens, max_new_tokens, batch_size, max_tokens, n_slots, max_seq_len):
+def plan_batches(prompt_lens, max_new_tokens, batch_size, max_tokens, n_slots, max_seq_len, ring_pages=0):
     """Splits the requests (in order) into batches that fit the cache: at most
     batch_size and n_slots sequences, and pages for every sequence at its longest
-    (prompt + new tokens, capped by the context).  Returns lists of indices."""
+    (prompt + new tokens, capped by the context).  ring_pages: the most pages that a sequence holds however long it grows (0: as many
+    as its tokens fill); counted for requests that would not fit otherwise.  Returns lists of indices."""
     limit = max(1, min(batch_size or n_slots, n_slots))
     budget = pages_for(max_tokens)
     out, cur, used = [], [], 0
@@ -56,6 +57,8 @@ def plan_batches(prompt_lens, max_new_tokens, batch_size, max_tokens, n_slots, m
         if n > max_seq_len:
             raise ValueError("request %d: a prompt of %d tokens does not fit the context of %d" % (i, n, max_seq_len))
         need = pages_for(min(n + max_new_tokens, max_seq_len))
+        if need > budget and ring_pages:
+            need = min(need, ring_pages)
         if need > budget:
             raise ValueError("request %d needs %d tokens of cache, the engine holds %d"
                              % (i, need * PAGE, budget * PAGE))
@@ -114,7 +117,7 @@ def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_
     if max_new_tokens <= 0 or not prompts:
         return results
     plan = plan_batches([len(p) for p in prompts], max_new_tokens, batch_size, engine.cache.n_pages * PAGE,
-                        engine.cache.n_slots, max_len)
+                        engine.cache.n_slots, max_len, getattr(engine.cache, "whole_rings", lambda: 0)())
     for batch in plan:
         stats.batches += 1
         stats.batch_sizes.append(len(batch))
