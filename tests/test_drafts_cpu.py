@@ -460,3 +460,31 @@ def test_a_step_s_drafts_stay_within_the_engine_s_limit(most):
     out = generate_drafted(engine, [[5] * (i + 1) for i in range(8)], max_new_tokens=300, stop_ids=[], sampler=ScriptedTokens(), guess=chain_guess, max_nodes=64)
     assert out == [[7 * r + s for s in range(300)] for r in range(8)]
     assert max(max(x) for x in engine.sizes) == min(64, (most or 1 << 30) // 8 if most != 17 else 2) and not engine.lens
+
+
+# ------------------------------------------------------------------------------------------------ models without drafts
+def _design(module):
+    return next(v for k, v in vars(module).items() if k.isupper() and isinstance(v, dict) and "layers" in v)
+
+
+def test_models_say_why_they_take_no_drafts():
+    """The reason is the layer's own: state, sinks, a term by the distance, or an arrangement around plain attention that offers none."""
+    import bovozen_configs
+    import gedunex_configs
+    import gemepel_configs
+    import situlorn_configs
+    import tiny_configs
+    import zebivik_configs
+    from yalm_amd import Model, config_from_dict
+    plain = config_from_dict(tiny_configs.ALL["tiny_llama"])
+    assert Model(plain.to_spec()).draft_refusal() == "" and Model(plain.to_spec()).takes_drafts()
+    sinks = Model(plain.with_context(20).to_spec())
+    assert not sinks.takes_drafts() and "layer 0" in sinks.draft_refusal() and "sinks" in sinks.draft_refusal()
+    said = {}
+    for module in (bovozen_configs, gedunex_configs, gemepel_configs, situlorn_configs, zebivik_configs):
+        model = Model(config_from_dict(_design(module)).to_spec())
+        said[module.__name__] = model.draft_refusal()
+        assert not model.takes_drafts() and said[module.__name__]
+    for name, why in (("gedunex", "ParallelResidualBlock"), ("gemepel", "embedding"), ("situlorn", "PostNormResidualBlock"), ("zebivik", "SandwichResidualBlock"),
+                      ("bovozen", "mixer")):
+        assert why in said[name + "_configs"], said

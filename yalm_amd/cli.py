@@ -179,7 +179,7 @@ def run_completion(a):
     from .generate import GenerationStats, generate
     model = _load(a)
     if a["draft"] and not model.takes_drafts():
-        error_usage("--draft is not offered for this model (its layers carry state, keep attention sinks or add a term by the distance)")
+        error_usage("--draft is not offered for this model (%s)" % model.draft_refusal())
     prompts, tok = _prompts(a, model)
     max_len = model.spec.max_positions
     steps = a["num_steps"]

@@ -285,8 +285,7 @@ class Engine:
         B = len(slots)
         starts = self._starts(slots)
         if not self.model.takes_drafts():
-            raise StepError("this model's layers do not take drafted tokens (they carry state from token to token, keep attention sinks or add a "
-                            "term by the distance)")
+            raise StepError("this model does not take drafted tokens (%s)" % self.model.draft_refusal())
         if len(tokens) != B or (parents is not None and len(parents) != B):
             raise StepError("slots, tokens and parents must have the same length")
         n_tok = [len(t) for t in tokens]

@@ -187,9 +187,18 @@ class Model:
     def takes_drafts(self):
         """Whether steps of drafted tokens can run: nothing but keys and values is kept of a sequence, and every block's mixer attends to
         trees of tokens (a block says so with `takes_drafts`)."""
+        return not self.draft_refusal()
+
+    def draft_refusal(self):
+        """Why they cannot ("": they can): what the first layer that is in the way says of itself, or that its arrangement says nothing."""
         if getattr(self.embedding, "cache_request", lambda: None)() is not None:
-            return False
-        return all(getattr(self.blocks[e.layer], "takes_drafts", False) for e in self.schedule)
+            return "the embedding keeps something of every sequence"
+        for e in self.schedule:
+            block = self.blocks[e.layer]
+            if not getattr(block, "takes_drafts", False):
+                return "layer %d: %s" % (e.layer, getattr(block, "draft_refusal", "") or "drafted tokens are not offered in its arrangement (%s)"
+                                         % type(block).__name__)
+        return ""
 
     def describe(self):
         """({line on the kernels that serve a part: the schedule entries it stands for}, the lines that

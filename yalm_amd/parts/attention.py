@@ -228,7 +228,14 @@ class GQAttention(Part):
     def takes_drafts(self):
         """Whether a step of drafted tokens (StepContext: mode 'draft') can run here: not beside sinks, which are stored as a sequence
         passes them, nor with a term by the distance, which attn_tree does not add."""
-        return not self.sinks and not hasattr(self.position, "score_bias")
+        return not self.draft_refusal
+
+    @property
+    def draft_refusal(self):
+        """Why it cannot ("": it can)."""
+        if self.sinks:
+            return "its attention keeps sinks"
+        return "its attention adds a term by the distance" if hasattr(self.position, "score_bias") else ""
 
     def fuses_norm(self, norm, x, ctx):
         if not hasattr(norm, "fused") or self.head_dim % 16:

@@ -36,6 +36,15 @@ class PreNormResidualBlock(Part):
         """Whether the layer runs in a step of drafted tokens: its mixer does, and no filter in front of it carries state."""
         return self.mixer_input is None and getattr(self.mixer, "takes_drafts", False)
 
+    @property
+    def draft_refusal(self):
+        """Why it does not ("": it does)."""
+        if self.takes_drafts:
+            return ""
+        if self.mixer_input is not None:
+            return "the filter in front of its mixer carries state from token to token"
+        return getattr(self.mixer, "draft_refusal", "") or "its mixer (%s) does not attend to trees of tokens" % type(self.mixer).__name__
+
     def cache_request(self):
         """What the layer keeps for a sequence: the mixer's, and beside it what the filter in front of the mixer keeps."""
         if self.mixer_input is None:
