@@ -513,3 +513,92 @@ def test_trees_in_a_graph_and_the_same_bits_twice(dtype):
         assert torch.equal(out, first)
     want, lim = tree_reference(c)
     assert ((first.cpu().double().view(53, 8, 128) - want).abs() <= lim).all()
+
+
+# ------------------------------------------------------------------------------------------------ trees over LDS, by how many columns a workgroup takes
+def columns_of(c):
+    """How many columns (nodes times the heads of a group) a workgroup of the bfloat16 kernels takes."""
+    cols = max(c["nodes"]) * (c["n_heads"] // c["n_kv"])
+    if cols <= 32 or c["hd"] % 32:
+        return 16 if cols <= 16 else 32
+    if cols <= 64:
+        return 64
+    units = torch.cuda.get_device_properties(0).multi_processor_count
+    return 256 if cols > 128 and 2 * len(c["nodes"]) * c["n_kv"] > units else 128
+
+
+@pytest.mark.parametrize("hd", [128, 32])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("splits", [None, 3])
+def test_trees_with_all_columns_in_one_workgroup(hd, window, splits):
+    """Sequences enough that more than 128 columns go in one workgroup: in one launch sequences that all eight waves share by columns, ones
+    that two groups of waves share by pages, ones of a single tile and ones without nodes; contexts from none to several pages."""
+    nodes = [61, 1, 33, 45, 0, 16, 61, 32, 5, 40, 48, 2, 61, 17, 34, 9, 58, 3, 37, 61, 20, 33, 64, 31]
+    held = [0, 1, 63, 64, 65, 127, 200, 300, 5, 129, 191, 400, 64, 2, 250, 33, 128, 90, 61, 3, 0, 150, 448, 320]
+    c = tree_case(held, nodes, 32, 8, hd, torch.bfloat16, window=window, seed=hd + window)
+    assert columns_of(c) == 256 and len(nodes) == len(held) == 24
+    check_tree(c, "hd %d window %d splits %s" % (hd, window, splits), splits=splits)
+
+
+FORMS = {64: (1, 4, 1, 12), 128: (2, 8, 2, 30), 1280: (2, 8, 2, 50), 256: (17, 32, 8, 45)}       # columns -> sequences, heads, KV heads, nodes; 1280: two workgroups of 128
+
+
+@pytest.fixture(scope="module")
+def lds_cases():
+    """Each form's case and what it gives, worked out once."""
+    made = {}
+
+    def get(form, hd):
+        if (form, hd) not in made:
+            B, heads, kv, nodes = FORMS[form]
+            held = [150] + [10 + 7 * b for b in range(1, B)]
+            c = tree_case(held, [nodes] * B, heads, kv, hd, torch.bfloat16, window=130, seed=form + hd)
+            assert columns_of(c) == {1280: 128}.get(form, form)
+            made[form, hd] = (c,) + tree_reference(c)
+        return made[form, hd]
+
+    return get
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("form", sorted(FORMS))
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_what_a_row_does_not_see_does_not_reach_it_over_lds(lds_cases, splits, bad, form, hd):
+    """As for few columns: a drafted token, one at the window's edge and one that every row sees, whose values (and keys) are no numbers,
+    on both of a round's pages: they reach the rows that see them and no other, and leave every other element as it is."""
+    c, want, lim = lds_cases(form, hd)
+    B, heads, kv, nodes = FORMS[form]
+    G = heads // kv
+    rows_of = list(tree_rows(c))
+    elements = [5, 6, 7, 8, hd - 1]
+    for pos in (150 + 3, 150 + nodes - 1, 22, 100):
+        rows = [r for r, (b, _, at) in enumerate(rows_of) if b == 0 and pos in at]
+        assert 0 < len(rows) and (pos != 100 or len(rows) == nodes)
+        free = sorted(set(range(len(rows_of))) - set(rows))
+        page = int(c["table"][c["slots"][0], pos // PAGE % c["ring"]])
+        g = kv - 1
+        e = dict(c, vp=c["vp"].clone())                        # the value alone
+        e["vp"][page, g, elements, pos % PAGE] = bad
+        got = run_tree(e, splits=splits)
+        assert torch.isfinite(got[free]).all() and ((got - want).abs() <= lim)[free].all(), (pos, "rows that do not see it")
+        odd = got[rows][:, g * G:][..., elements]
+        assert (torch.isnan(odd) if bad != bad else odd == bad).all(), (pos, "rows that see it")
+        rest = got[rows].clone()
+        for x in elements:
+            rest[:, g * G:, x] = want[rows][:, g * G:, x]
+        assert ((rest - want[rows]).abs() <= lim[rows]).all(), (pos, "the other elements")
+        d = dict(e, kp=c["kp"].clone())                        # the key too
+        d["kp"][page, g, pos % PAGE] = bad
+        got = run_tree(d, splits=splits)
+        assert torch.isfinite(got[free]).all() and ((got - want).abs() <= lim)[free].all(), (pos, "keys")
+        assert not torch.isfinite(got[rows][:, g * G:]).all(dim=-1).any()
+
+
+def test_the_splits_count_this_card_s_units():
+    """attn_tree_splits has the compute units written out that the kernels' own choice of columns asks the card for."""
+    assert torch.cuda.get_device_properties(0).multi_processor_count == 256
+    for B in (16, 17):                                         # 2 x 16 x 8 halves all run at once, 2 x 17 x 8 do not
+        c = dict(nodes=[61] * B, n_heads=32, n_kv=8, hd=128)
+        chunks = -(-61 * 4 // columns_of(c))
+        assert K().attn_tree_splits(B, 61, 100000, 32, 8, 128, torch.bfloat16) == max(1, 256 // (B * 8 * chunks))
