@@ -418,7 +418,8 @@ class CacheManager:
         if not self.unbounded and max(new_lens) > self.max_seq_len:
             raise CacheFull("a sequence of %d tokens exceeds the longest the cache holds (%d)"
                             % (max(new_lens), self.max_seq_len))
-        for g in self._short:
+        outgrown = [g for g in self._short if max(new_lens) > g.ring_pages * PAGE]
+        for g in outgrown:
             for s, o, n in zip(slots, old_lens, n_new):
                 if o > 0 and n > g.room(s, o):
                     raise CacheFull("a sequence of %d tokens cannot go on by %d: the cache's %d pages do not hold all that a window of %d positions "
@@ -438,7 +439,7 @@ class CacheManager:
                 g.grow(g_slots, g_old, g_new)
         for g in self.kv_groups:
             g.flush()
-        for g in self._short:
+        for g in outgrown:
             for s, o, n in zip(slots, old_lens, new_lens):
                 g.note(s, o, n)
         for s, nl in zip(slots, new_lens):
