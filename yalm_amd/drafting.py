@@ -3,14 +3,17 @@ it would have drawn behind each of them, and the path of guesses that it agrees 
 
 The tokens are those of generate() with the same seed, up to rounding: the token of a place is drawn from the model's own logits there, with
 the number that belongs to the request and the place, and a guess is kept only if it is that token.  A guesser that is never right
-costs a step of wider rows a token; each guess that is right saves a step."""
+costs a step of wider rows a token, launched kernel by kernel, and its own time on the host; each guess that is right saves a step.  At the Mistral-7B
+shape in bfloat16, 8 nodes, tokens a second behind 3,000 tokens: one sequence 254 with the text's own guesses where none is right and 2,227 with ones that
+always are (generate: 362), eight sequences 1,120 where few are (2,440)."""
 from .cache.manager import PAGE
 from .generate import GenerationStats, plan_batches
 
 
 def lookup_tree(history, n, longest=3, branches=3):
     """Guesses at what follows `history`, from history itself: what followed the places where its last tokens (the last `longest`, else
-    fewer) stood before, the latest ones first.  Returns (tokens, parents) of a tree of at most n nodes whose root is history's last token."""
+    fewer) stood before, the latest ones first.  Returns (tokens, parents) of a tree of at most n nodes whose root is history's last token.
+    It looks through the whole text, up to three times: 0.5 ms for 3,000 tokens that say nothing, 4.6 for 28,000."""
     tokens, parents = [history[-1]], [-1]
     children = {}                                     # (node, token) -> node
     last = len(history) - 1

@@ -77,7 +77,7 @@ def generate(engine, prompts, max_new_tokens=256, temperature=0.0, seed=0, stop_
     """Generates for every prompt (a list of token ids).  Returns the new tokens of
     each request, in the order of the prompts.  top_k, top_p, min_p: see Sampler.draw, here one number
     for all requests, as the temperature is.  samples > 1: every prompt is answered that many
-    times and runs once (its sequence is forked behind the prompt step); the answers of prompt i are the requests samples * i, samples * i + 1,
+    times and runs once in every batch that has answers to it (its sequence is forked behind the prompt step); the answers of prompt i are the requests samples * i, samples * i + 1,
     ... of the result and of on_token, drawn as requests of the ids samples * id, samples * id + 1, ...  stop_ids None means the model's own
     (config eos); on_token(request index, token) is called for every new token.
     ahead: queue each step before the host has read the tokens of the step before

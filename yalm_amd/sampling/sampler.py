@@ -116,7 +116,7 @@ class Sampler:
     def draw(self, logits, temperature, request_ids, steps, top_k=0, top_p=1.0, min_p=0.0):
         """One token for each row of logits [R, vocab] (device, float32); temperature 0 is argmax.  top_k (0: off), top_p (1: off) and
         min_p (0: off) leave a part of the tokens to draw from (kernels.sample_filtered); they and the temperature are numbers for all rows
-        or sequences of one for each.
+        or sequences of one for each.  A refused draw changes nothing; draws may be queued on several streams, each behind what made its logits.
         Nothing waits for the device here: the tokens can feed the next step from where they lie
         while the host reads them a step later."""
         R = logits.shape[0]
