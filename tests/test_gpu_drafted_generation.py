@@ -404,3 +404,83 @@ def test_the_command_line_runs_a_text_past_its_context(folders, capsys):
     main([folders["tiny_mistral"], "--tokens", "1,17,200", "-n", "500", "-t", "0", "-T", "24", "--dtype", "float32"])
     stop = tiny_configs.ALL["tiny_mistral"].get("eos_token_id")
     assert " ".join(map(str, want[:want.index(stop) + 1] if stop in want else want)) in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("name,changes,max_tokens,seed", [("tiny_llama3", {}, 640, 1), ("tiny_llama3", {}, 1280, 2), ("tiny_mistral", {"sliding_window": 70, "max_position_embeddings": 300}, 1280, 3),
+                                                         ("tiny_mistral", {"sliding_window": 100, "max_position_embeddings": 128}, 640, 4),
+                                                         ("tiny_mistral", {"sliding_window": 150, "max_position_embeddings": 300}, 128, 5)])
+def test_random_use_of_prompts_steps_trees_and_forks(tmp_path, name, changes, max_tokens, seed):
+    """Sequences that start, go on by a token or a tree, keep any path of it, fork and end, in any order, in a cache that is often full:
+    every logit is that of the sequence's own text, and what is refused changes nothing."""
+    from yalm_amd import Engine, Model, StepError
+    cfg = {**tiny_configs.ALL[name], **changes}
+    folder = helpers.make_folder(tmp_path, name, cfg, seed=8)
+    engine = Engine(Model.from_folder(folder, dtype=torch.float32, device="cuda:0"), max_tokens=max_tokens, max_batch=5, max_draft=24)
+    rng = np.random.default_rng(seed)
+    V, depth = cfg["vocab_size"], engine.max_draft_depth
+    texts, done, refused = {}, {}, 0
+
+    def books():
+        return list(engine.cache.seq_len), sorted(engine.cache.slots.held), [(g.pool.n_free, g.table_host.tolist()) for g in engine.cache.kv_groups]
+
+    def check(logits, text, what):
+        helpers.check_logits(logits.float().cpu().numpy()[None], helpers.plain_logits(folder, tuple(text), "float32")[-1:], "float32", what)
+
+    for turn in range(110):
+        kind = rng.choice(["start", "step", "step", "tree", "tree", "tree", "fork", "end"], p=[0.12, 0.1, 0.1, 0.18, 0.18, 0.18, 0.08, 0.06])
+        some = [s for s in texts if rng.random() < 0.7] or list(texts)[:1]
+        before = books()
+        try:
+            if kind == "start":
+                n = int(rng.choice([1, 5, 63, 64, 65, 100, 120]))
+                (s,) = engine.start(1)
+                text = rng.integers(0, V, n).tolist()
+                try:
+                    check(engine.step([s], [text])[0], text, "turn %d: prompt of %d" % (turn, n))
+                    texts[s] = text
+                finally:
+                    if s not in texts:
+                        engine.release([s])
+            elif kind == "step" and some:
+                new = [[int(rng.integers(0, V))] for _ in some]
+                logits = engine.step(some, new)
+                for i, s in enumerate(some):
+                    texts[s] = texts[s] + new[i]
+                    check(logits[i], texts[s], "turn %d: step" % turn)
+            elif kind == "tree" and some:
+                sizes = [int(rng.integers(1, 25)) for _ in some]
+                trees = [tree(n, turn + n) for n in sizes]
+                tokens = [rng.integers(0, V, n).tolist() for n in sizes]
+                logits = engine.draft_step(some, tokens, trees)
+                row, paths = 0, []
+                for i, s in enumerate(some):
+                    for j in {0, sizes[i] - 1, int(rng.integers(0, sizes[i]))}:
+                        check(logits[row + j], texts[s] + [tokens[i][k] for k in path_to(trees[i], j)], "turn %d: node %d" % (turn, j))
+                    row += sizes[i]
+                    paths.append(path_to(trees[i], int(rng.integers(0, sizes[i]))) if rng.random() < 0.9 else [])
+                engine.keep(some, paths)
+                for i, s in enumerate(some):
+                    texts[s] = texts[s] + [tokens[i][j] for j in paths[i]]
+            elif kind == "fork" and texts:
+                s = list(texts)[int(rng.integers(0, len(texts)))]
+                for t in engine.fork(s, int(rng.integers(1, 3))):
+                    texts[t] = list(texts[s])
+            elif kind == "end" and texts:
+                s = list(texts)[int(rng.integers(0, len(texts)))]
+                engine.release([s])
+                del texts[s]
+            else:
+                continue
+            done[kind] = done.get(kind, 0) + 1
+        except (StepError, RuntimeError) as e:
+            assert any(w in str(e) for w in ("pages", "slots", "position", "longest", "window")), e
+            assert books()[:2] == before[:2] and [f for f, _ in books()[2]] == [f for f, _ in before[2]]
+            refused += 1
+            if texts and rng.random() < 0.5:                   # make room
+                s = list(texts)[0]
+                engine.release([s])
+                del texts[s]
+        assert all(engine.length(s) == len(t) for s, t in texts.items())
+    assert refused > 0 and len(done) == 5 and depth >= 24, (done, refused)
+    engine.release(list(texts))
+    assert all(g.pool.n_free == g.n_pages for g in engine.cache.kv_groups)

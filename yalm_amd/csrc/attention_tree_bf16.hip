@@ -20,7 +20,7 @@ int tree_columns(int B, int max_nodes, int n_heads, int n_kv_heads, int head_dim
 // of consecutive bytes), the next two in flight while these are multiplied.  A round of two pages against 128 columns of 128 elements takes 2.0 us, where
 // the vector units want 1.07 (322 instructions a wave, two waves a unit), the matrix cores 0.85 and LDS 1.07: with 128 KB of pages a compute unit holds
 // one workgroup, whose waves meet at a barrier a round and wait for the pages of the next.
-// One sequence of 28,000 tokens and 61 nodes 46 us (2.5 TB/s, 600 TFLOP/s), 64 of up to 3,041 and 40 nodes 146 to 157 (3.7 to 3.9 TB/s).  With up to 64 NC columns
+// One sequence of 28,000 tokens and 61 nodes 46 us (2.5 TB/s, 600 TFLOP/s), 64 of up to 3,041 and 40 nodes 146 to 160 (3.6 to 3.9 TB/s).  With up to 64 NC columns
 // two groups of four waves take a page each and the second hands its results to the first at the end; with more (`wide`, up
 // to 128 NC) all eight waves split the columns and take both pages.  A wave has the tiles wave, wave + 4 (wide: + 8), ... of 16
 // columns, and leaves out those that the sequence does not fill.
